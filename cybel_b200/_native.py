@@ -47,6 +47,7 @@ _ip = ctypes.POINTER(ctypes.c_int)
 _vpp = ctypes.POINTER(ctypes.c_void_p)
 _fpp = ctypes.POINTER(ctypes.POINTER(ctypes.c_float))
 _f = ctypes.c_float
+_d = ctypes.c_double
 SIGNATURES.update(
     {
         "simd_repack_q4k_r4": ([_vp, _vp, _i, _i], _i),
@@ -81,6 +82,13 @@ SIGNATURES.update(
                                                _i, _vp, _i, _vp, _vp, _i, _ll, _ll, _vp], _i),
         "b200q_rope_attention_decode_tokens": ([_vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _f, _vp, _vp, _i, _vp, _vp, _i,
                                                 _ll, _ll, _vp], _i),
+        "b200q_rope_table": ([_i, _d, _i, _d, _d, _d, _i,
+                              ctypes.POINTER(ctypes.c_ulonglong), ctypes.POINTER(ctypes.c_double)], _i),
+        "b200q_rope_rows": ([_vp, _vp, _i, _i, _i, _i, _ll, _ll, _vp, _vp, _i, _i, _d, _vp], _i),
+        "b200q_rope_append_paged": ([_vp, _vp, _vp, _i, _i, _i, _vp, _vp, _i, _i, _i, _ll, _ll, _vp, _ll, _vp, _i, _i,
+                                     _d, _i, _vp, _vp, _vp, _vp, _i, _i, _vp, _i, _vp], _i),
+        "b200q_attention_paged": ([_vp, _i, _i, _i, _vp, _vp, _i, _i, _i, _i, _i, _ll, _vp, _ll, _f, _f, _vp, _i, _vp,
+                                   _i, _vp, _vp, _vp, _vp, _i, _i, _vp, _i, _vp], _i),
         "b200q_swiglu_q": ([_vp, _vp, _vp, _i, _i, _vp], _i),
         "b200q_swiglu_rows": ([_vp, _vp, _i, _i, _vp], _i),
         "b200q_matmul_xq": ([_i, _i, _vp, _vp, _vp, _i, _i, _i, ctypes.c_float, ctypes.c_float, _i, _vp], _i),
@@ -144,6 +152,9 @@ def check(status: int, what: str) -> None:
 STATUS_TIMEOUT = 1  # device status bit: a kernel's bounded wait gave up
 STATUS_BAD_PAGE = 2  # device status bit: a paged cache's table named no page or one outside the pool
 KV_F16, KV_Q8 = 0, 1  # paged KV storage modes
+F32, F16 = 0, 1  # element types of the ragged operators' rows
+ROPE_LAYOUTS = {"interleaved": 0, "half": 1}
+ROPE_SCALINGS = {"none": 0, "linear": 1, "llama3": 2, "yarn": 3}
 
 
 def check_device(device: int, what: str = "device status") -> None:

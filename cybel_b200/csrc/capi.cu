@@ -1035,6 +1035,70 @@ void simd_fused_moe_ffn(const float* x, int in_dim, const int* expert_indices, c
     set_last_error(rc);
 }
 
+// ---- ragged batches over a paged cache ----------------------------------------
+int b200q_rope_table(int rot_dim, double theta, int scaling, double factor, double low, double high,
+                     int original_context, unsigned long long* turns, double* mag) {
+    const int rc = rope_table(rot_dim, theta, scaling, factor, low, high, original_context, turns, mag);
+    set_last_error(rc);
+    return rc;
+}
+
+int b200q_rope_rows(const void* x, void* out, int dtype, int n_rows, int heads, int head_dim, long long x_stride,
+                    long long out_stride, const int* positions, const unsigned long long* turns, int rot_dim,
+                    int layout, double mag, void* stream) {
+    Device* dev = nullptr;
+    int rc = current_device_state(&dev);
+    if (rc == B200Q_OK)
+        rc = launch_rope_rows(x, out, dtype, n_rows, heads, head_dim, x_stride, out_stride, positions, turns, rot_dim,
+                              layout, mag, dev, static_cast<cudaStream_t>(stream));
+    set_last_error(rc);
+    return rc;
+}
+
+int b200q_rope_append_paged(const void* q, const void* k, const void* v, int dtype, int n_tokens, int batch,
+                            const int* cu_q, const int* kv_len, int n_heads, int n_kv_heads, int head_dim,
+                            long long q_stride, long long kv_stride, void* q_out, long long q_out_stride,
+                            const unsigned long long* turns, int rot_dim, int layout, double mag, int kv_mode,
+                            void* k_pages, void* v_pages, float* k_scales, float* v_scales, int n_slots, int page_size,
+                            const int* page_table, int pages_per_seq, void* stream) {
+    Device* dev = nullptr;
+    int rc = current_device_state(&dev);
+    const PagedKV kv{kv_mode, k_pages,   v_pages,    k_scales,      v_scales,
+                     n_slots, page_size, page_table, pages_per_seq, n_kv_heads};
+    if (rc == B200Q_OK)
+        rc = launch_rope_append(q, k, v, dtype, n_tokens, batch, cu_q, kv_len, n_heads, head_dim, q_stride, kv_stride,
+                                q_out, q_out_stride, turns, rot_dim, layout, mag, kv, dev,
+                                static_cast<cudaStream_t>(stream));
+    set_last_error(rc);
+    return rc;
+}
+
+int b200q_attention_paged(const void* q, int dtype, int n_tokens, int batch, const int* cu_q, const int* kv_len,
+                          int max_q_len, int max_kv_len, int n_heads, int n_kv_heads, int head_dim, long long q_stride,
+                          void* out, long long out_stride, float scale, float softcap, const float* slopes, int window,
+                          const int* prefix, int kv_mode, const void* k_pages, const void* v_pages,
+                          const float* k_scales, const float* v_scales, int n_slots, int page_size,
+                          const int* page_table, int pages_per_seq, void* stream) {
+    Device* dev = nullptr;
+    int rc = current_device_state(&dev);
+    const PagedKV kv{kv_mode,
+                     const_cast<void*>(k_pages),
+                     const_cast<void*>(v_pages),
+                     const_cast<float*>(k_scales),
+                     const_cast<float*>(v_scales),
+                     n_slots,
+                     page_size,
+                     page_table,
+                     pages_per_seq,
+                     n_kv_heads};
+    if (rc == B200Q_OK)
+        rc = launch_attention_paged(q, dtype, n_tokens, batch, cu_q, kv_len, max_q_len, max_kv_len, n_heads, head_dim,
+                                    q_stride, out, out_stride, scale, softcap, slopes, window, prefix, kv, dev,
+                                    static_cast<cudaStream_t>(stream));
+    set_last_error(rc);
+    return rc;
+}
+
 // ---- controls ----------------------------------------------------------------
 int b200q_set_act_mode(int act_mode) {
     const int prev = act_mode_now();

@@ -128,6 +128,31 @@ int launch_rope_attention_paged(const float* q, const float* k, const float* v, 
                                 float* k_scales, float* v_scales, int n_slots, int page_size, const int* page_table,
                                 int pages_per_seq, float* out, void* xq, int act_mode, Device* dev, cudaStream_t st,
                                 long long q_stride = 0, long long kv_stride = 0);
+// Ragged batches over a paged cache (ragged.cu, attn_ragged.cu).
+struct PagedKV {
+    int kv_mode;
+    void *k_pages, *v_pages;
+    float *k_scales, *v_scales;
+    int n_slots, page_size;
+    const int* page_table;
+    int pages_per_seq, n_kv;
+};
+struct PagedView;
+int check_paged(const PagedKV& p, int hd);
+PagedView paged_view(const PagedKV& p, Device* dev);
+int rope_table(int rot_dim, double theta, int scaling, double factor, double low, double high, int original_context,
+               unsigned long long* turns, double* mag);
+int launch_rope_rows(const void* x, void* out, int dtype, int rows, int heads, int hd, long long x_stride,
+                     long long out_stride, const int* positions, const unsigned long long* turns, int rot, int layout,
+                     double mag, Device* dev, cudaStream_t st);
+int launch_rope_append(const void* q, const void* k, const void* v, int dtype, int n_tokens, int batch, const int* cu_q,
+                       const int* kv_len, int heads, int hd, long long q_stride, long long kv_stride, void* q_out,
+                       long long q_out_stride, const unsigned long long* turns, int rot, int layout, double mag,
+                       const PagedKV& pkv, Device* dev, cudaStream_t st);
+int launch_attention_paged(const void* q, int dtype, int n_tokens, int batch, const int* cu_q, const int* kv_len,
+                           int max_q_len, int max_kv_len, int heads, int hd, long long q_stride, void* out,
+                           long long out_stride, float scale, float softcap, const float* slopes, int window,
+                           const int* prefix, const PagedKV& pkv, Device* dev, cudaStream_t st);
 int launch_swiglu(const float* g, const float* u, float* out, long long n, cudaStream_t st);
 // SiLU(gate) * up for `rows` rows of [gate n | up n] (b200q_swiglu_rows).
 int launch_swiglu_rows(const float* gu, float* out, int rows, int n, cudaStream_t st);

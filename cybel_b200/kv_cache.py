@@ -11,7 +11,9 @@ execution checkpoint (model_graph.cpp:4725-4776).
 Here every page lives in one preallocated pool per cache (keys, values and,
 in Q8 mode, their scales), and a page table ``[layer][sequence][page]`` of
 int32 slots (-1: no page) tells the attention kernel
-(b200q_rope_attention_decode_paged) where each position is. Pages of a
+(b200q_rope_attention_decode_paged) where each position is. ``append`` and
+``attend`` serve batches whose sequences differ in length (RaggedBatch,
+RopeTable in paged_attention.py). Pages of a
 sequence are assigned from a free list when ``ensure(pos)`` first meets them,
 so the pool can be smaller than layers x sequences x max_seq positions. fp16
 replaces the reference's fp32 pages (the contiguous decode cache stores fp16
@@ -29,7 +31,8 @@ import numpy as np
 from . import _native
 
 KV_PAGE_SIZE = 4096  # positions per page (model_graph.cpp:317)
-HEAD_DIM = 128       # the attention kernels' head size
+HEAD_DIM = 128       # head size of the one-position attention (``PagedKVCache.attention``)
+HEAD_DIMS = (64, 128)  # head sizes of ``append`` and ``attend``
 
 
 def q8_from_env(env: Mapping[str, str] | None = None) -> bool:
@@ -70,8 +73,8 @@ class PagedKVCache:
         the pools on the host: page bookkeeping only, no attention calls)."""
         import torch
 
-        if head_dim != HEAD_DIM:
-            raise ValueError("the attention kernels are built for head_dim 128")
+        if head_dim not in HEAD_DIMS:
+            raise ValueError("the attention kernels are built for head_dim 64 and 128")
         if min(layers, kv_heads, max_seq, batch, page_size) <= 0:
             raise ValueError("layers, kv_heads, max_seq, batch and page_size must be positive")
         self.layers, self.kv_heads, self.batch = layers, kv_heads, batch
@@ -130,6 +133,30 @@ class PagedKVCache:
         for p in range(pages.start, pages.stop):
             for li, b in np.argwhere(self.table_host[:, :, p] < 0):
                 self.table_host[li, b, p] = self._free.pop()
+        self.table.copy_(torch.from_numpy(self.table_host))
+
+    def ensure_batch(self, batch) -> None:
+        """Give every layer the pages that a ragged batch's tokens fall in
+        (paged_attention.RaggedBatch, one sequence per sequence of the cache),
+        as ``ensure`` does for all sequences at one position. Raises
+        MemoryError, with nothing assigned, when the pool has too few."""
+        import torch
+
+        if batch.batch != self.batch:
+            raise ValueError("the ragged batch has another number of sequences than the cache")
+        if max(batch.kv_lens) > self.max_seq:
+            raise ValueError("position outside the cache")
+        new = []
+        for b, (q, n) in enumerate(zip(batch.q_lens, batch.kv_lens)):
+            if q:
+                pages = slice((n - q) // self.page_size, (n - 1) // self.page_size + 1)
+                new += [(li, b, pages.start + p) for li, p in np.argwhere(self.table_host[:, b, pages] < 0)]
+        if not new:
+            return
+        if len(new) > len(self._free):
+            raise MemoryError(f"KV page pool exhausted ({self.n_slots} pages, {len(self._free)} free, {len(new)} needed)")
+        for li, b, p in new:
+            self.table_host[li, b, p] = self._free.pop()
         self.table.copy_(torch.from_numpy(self.table_host))
 
     def assign(self, layer: int, seq: int, page: int, slot: int) -> None:
@@ -198,6 +225,42 @@ class PagedKVCache:
             q, k, v, self.batch, n_tokens, n_heads, self.kv_heads, self.head_dim, pos, theta, self.kv_mode, self.k.data_ptr(),
             self.v.data_ptr(), ks, vs, self.n_slots, self.page_size, self.table_ptr(layer), self.pages_per_seq, out,
             xq, act_mode, q_stride, kv_stride, stream), "paged attention")
+
+    def _pools(self, layer: int) -> tuple:
+        if not 0 <= layer < self.layers:
+            raise ValueError("layer outside the cache")
+        q8 = self.q8
+        return (self.kv_mode, self.k.data_ptr(), self.v.data_ptr(), self.ks.data_ptr() if q8 else None,
+                self.vs.data_ptr() if q8 else None, self.n_slots, self.page_size, self.table_ptr(layer),
+                self.pages_per_seq)
+
+    def append(self, layer: int, k, v, batch, rope=None, q=None, q_out=None):
+        """Write a ragged batch's keys and values into layer `layer`, keys
+        rotated by `rope` (paged_attention.RopeTable; None: as they are), and
+        return the rotated queries (``q_out``, or a new tensor; None without
+        ``q``). k and v [n_tokens][kv_heads][head_dim] and q [n_tokens][heads]
+        [head_dim], fp32 or fp16, heads packed, rows any distance apart (the
+        parts of one projection output); q_out may be q. The pages of the
+        batch's positions must have been ensured (``ensure_batch``). Current
+        stream; b200q_rope_append_paged."""
+        from .paged_attention import append
+
+        return append(self, layer, k, v, batch, rope, q, q_out)
+
+    def attend(self, layer: int, q, batch, out=None, scale: float | None = None, softcap: float = 0.0, slopes=None,
+               window: int = 0, prefix=None):
+        """Attention of a ragged batch's rotated query rows over layer
+        `layer`, which holds the batch's own tokens already (``append``).
+        Scores q . k * scale (default 1 / sqrt(head_dim)), capped to
+        softcap * tanh(score / softcap) when softcap > 0, less
+        slopes[h] * distance (fp32 [heads]) when slopes are given; causal,
+        within the last `window` positions when window > 0, plus the first
+        prefix[b] positions (int32 [sequences]) for every row. q [n_tokens]
+        [heads][head_dim] fp32 or fp16; returns ``out`` (or a new tensor) of
+        q's type and shape. Current stream; b200q_attention_paged."""
+        from .paged_attention import attend
+
+        return attend(self, layer, q, batch, out, scale, softcap, slopes, window, prefix)
 
     def rows(self, layer: int, seq: int, kv_head: int, p0: int, p1: int):
         """Stored (codes or fp16 values, scales or None) of positions p0..p1-1

@@ -66,6 +66,19 @@ extern "C" {
 #define B200Q_KV_F16 0         /* fp16 pages */
 #define B200Q_KV_Q8 1          /* int8 pages + one fp32 scale per (position, kv head) */
 
+/* element types of the ragged operators' activation rows */
+#define B200Q_F32 0
+#define B200Q_F16 1
+
+/* rotary layouts: pairs (2p, 2p + 1), or (p, p + rot_dim / 2) */
+#define B200Q_ROPE_INTERLEAVED 0
+#define B200Q_ROPE_HALF 1
+/* frequency scalings of b200q_rope_table */
+#define B200Q_ROPE_PLAIN 0
+#define B200Q_ROPE_LINEAR 1
+#define B200Q_ROPE_LLAMA3 2
+#define B200Q_ROPE_YARN 3
+
 /* status codes */
 #define B200Q_OK 0
 #define B200Q_EINVAL (-1)      /* null pointer, non-positive size */
@@ -341,6 +354,77 @@ B200Q_API int b200q_rope_attention_decode_paged(const float* q, const float* k, 
                                                 float* k_scales, float* v_scales, int n_slots, int page_size,
                                                 const int* page_table, int pages_per_seq, float* out, void* xq,
                                                 int act_mode, long long q_stride, long long kv_stride, void* stream);
+
+/* ---------------------------------------------------------------------
+ * Ragged batches over a paged cache: sequences of different lengths in one
+ * call, from one new token each (a decode step) to whole prompts. Activation
+ * rows are fp32 or fp16 (dtype B200Q_F32 / B200Q_F16), one row per new token,
+ * sequence after sequence: rows cu_q[b] .. cu_q[b + 1] - 1 belong to sequence
+ * b, and the last of them sits at position kv_len[b] - 1 (token t of q_len at
+ * kv_len[b] - q_len + t). cu_q ([batch + 1], not falling) and kv_len ([batch])
+ * are device int32 arrays that only the kernels read, so a captured graph
+ * replays with the lengths they hold then. Rows that cu_q gives to no
+ * sequence are neither read nor written; a sequence may have no rows.
+ * Strides count elements between consecutive rows (0: packed). The paged
+ * cache is that of b200q_rope_attention_decode_paged, head_dim 64 or 128.
+ * ------------------------------------------------------------------- */
+
+/* The rotary table: turns[p], p < rot_dim / 2, is pair p's frequency
+ * theta^(-2p / rot_dim) / (2 pi), scaled, in units of 2^-64 turns per position
+ * (a host array; the kernels take a device copy). scaling B200Q_ROPE_PLAIN;
+ * _LINEAR: divided by factor; _LLAMA3: divided by factor where the pair makes
+ * fewer than `low` turns over original_context positions, kept above `high`
+ * turns, interpolated between; _YARN: interpolated over the pairs between the
+ * ones that make `high` and `low` turns, and *mag, the factor on cos and sin,
+ * 0.1 ln(factor) + 1 (1 otherwise). rot_dim even, at most 256; theta > 1. */
+B200Q_API int b200q_rope_table(int rot_dim, double theta, int scaling, double factor, double low, double high,
+                               int original_context, unsigned long long* turns, double* mag);
+
+/* out = x with the first rot_dim elements of each of `heads` heads rotated to
+ * positions[row] >= 0 (device int32), the others copied; out may be x. turns:
+ * device table of b200q_rope_table. Angles are exact to fp32 at any position. */
+B200Q_API int b200q_rope_rows(const void* x, void* out, int dtype, int n_rows, int heads, int head_dim,
+                              long long x_stride, long long out_stride, const int* positions,
+                              const unsigned long long* turns, int rot_dim, int layout, double mag, void* stream);
+
+/* Writes the rows' keys and values into the cache at their positions, keys
+ * rotated (turns NULL with rot_dim 0: as they are), and the rotated queries to
+ * q_out (NULL: no queries; may be q). k and v rows kv_stride elements apart.
+ * fp16 pages hold the rows rounded to fp16, Q8 pages the codes and scales of
+ * b200q_rope_attention_decode_paged (keys rotated in fp64 first, so that the
+ * codes are those of the exact rotation rounded to fp32). The pages of the
+ * positions are assigned before the call, each to one sequence; a row whose
+ * position has no page (or is negative) is not stored and sets device status
+ * bit 2. */
+B200Q_API int b200q_rope_append_paged(const void* q, const void* k, const void* v, int dtype, int n_tokens, int batch,
+                                      const int* cu_q, const int* kv_len, int n_heads, int n_kv_heads, int head_dim,
+                                      long long q_stride, long long kv_stride, void* q_out, long long q_out_stride,
+                                      const unsigned long long* turns, int rot_dim, int layout, double mag, int kv_mode,
+                                      void* k_pages, void* v_pages, float* k_scales, float* v_scales, int n_slots,
+                                      int page_size, const int* page_table, int pages_per_seq, void* stream);
+
+/* Attention of the batch's (rotated) query rows over the cache. For the row
+ * at position i and query head h (kv head h / (n_heads / n_kv_heads)):
+ *   s_j = scale q . k_j;  s_j = softcap tanh(s_j / softcap) if softcap > 0;
+ *   s_j -= slopes[h] |i - j| if slopes (device, [n_heads]) is given;
+ *   out = sum_j softmax(s)_j v_j over the visible j,
+ * j visible when j < kv_len[b], its page is assigned, and either j <= i with
+ * i - j < window (window 0: no limit) or j < prefix[b] (device int32 [batch],
+ * or NULL). Pages that no row sees need not be assigned (entry -1); an entry
+ * outside the pool, or a visible position past the table, hides the position
+ * and sets device status bit 2. A row that sees nothing is written as zeros.
+ * Non-finite keys or values reach only the rows that see them. max_q_len and
+ * max_kv_len, upper bounds of the sequences' rows and of kv_len, choose the
+ * kernel and how the keys are split; rows of a sequence past max_q_len may be
+ * left unwritten. scale > 0. q and out 16-byte aligned, strides a multiple of 16 bytes. */
+B200Q_API int b200q_attention_paged(const void* q, int dtype, int n_tokens, int batch, const int* cu_q,
+                                    const int* kv_len, int max_q_len, int max_kv_len, int n_heads, int n_kv_heads,
+                                    int head_dim, long long q_stride, void* out, long long out_stride, float scale,
+                                    float softcap, const float* slopes, int window, const int* prefix, int kv_mode,
+                                    const void* k_pages, const void* v_pages, const float* k_scales,
+                                    const float* v_scales, int n_slots, int page_size, const int* page_table,
+                                    int pages_per_seq, void* stream);
+
 B200Q_API int b200q_swiglu_q(const float* gate, const float* up, void* xq, int act_mode, int n, void* stream);
 /* out[r][j] = silu(gate_up[r][j]) * gate_up[r][n + j] for `rows` rows of one
  * gate|up projection output ([gate n | up n] per row): the SwiGLU step of a
