@@ -8,28 +8,16 @@
 //
 // j is visible when j < kv_len, its page is assigned, and j <= i with
 // i - j < window (window > 0), or j < prefix_b. A row that sees nothing is 0.
+#include <algorithm>
 #include <cmath>
 #include <type_traits>
 
+#include "attn_ragged.cuh"
 #include "internal.h"
-#include "ragged.cuh"
 
 namespace b200q {
 
 namespace {
-
-struct AttnArgs {
-    RaggedView r;
-    PagedView kv;
-    const void* q;
-    void* out;
-    const float* slopes;  // [heads] or NULL
-    const int* prefix;    // [batch] or NULL
-    long long q_stride, out_stride;
-    int heads;
-    int window;
-    float scale, cap;
-};
 
 __device__ __forceinline__ float4 kv_quad(const __half* p) {
     const uint2 x = *reinterpret_cast<const uint2*>(p);
@@ -58,6 +46,7 @@ __global__ void __launch_bounds__(128) b200q_attn_rows_kernel(const AttnArgs a) 
     const int b = seq_of_row(a.r, row);
     if (b < 0) return;
     const int2 rr = seq_rows(a.r, b);
+    if ((rr.y - rr.x) * a.group <= a.few_rows) return;
     const int n = a.r.kv_len[b];
     const int pos = n - (rr.y - row);
     const int kvh = head / (a.heads / a.kv.n_kv);
@@ -131,6 +120,10 @@ __global__ void __launch_bounds__(128) b200q_attn_rows_kernel(const AttnArgs a) 
 
 }  // namespace
 
+// Sequences with at most this many rows (tokens x query heads per kv head)
+// are the few-row kernel's.
+constexpr int kFewRows = 64;
+
 int launch_attention_paged(const void* q, int dtype, int n_tokens, int batch, const int* cu_q, const int* kv_len,
                            int max_q_len, int max_kv_len, int heads, int hd, long long q_stride, void* out,
                            long long out_stride, float scale, float softcap, const float* slopes, int window,
@@ -155,7 +148,7 @@ int launch_attention_paged(const void* q, int dtype, int n_tokens, int batch, co
         (reinterpret_cast<uintptr_t>(kv_len) & 3) || (reinterpret_cast<uintptr_t>(slopes) & 3) ||
         (reinterpret_cast<uintptr_t>(prefix) & 3))
         return B200Q_EALIGN;
-    if (n_tokens == 0) return B200Q_OK;
+    if (n_tokens == 0 || max_q_len == 0) return B200Q_OK;
     AttnArgs a{};
     a.r = RaggedView{cu_q, kv_len, batch, n_tokens};
     a.kv = paged_view(pkv, dev);
@@ -169,7 +162,14 @@ int launch_attention_paged(const void* q, int dtype, int n_tokens, int batch, co
     a.window = window;
     a.scale = scale;
     a.cap = softcap;
+    a.group = heads / pkv.n_kv;
+    while ((1ll << a.page_shift) < pkv.page_size) ++a.page_shift;
+    a.page_mul = static_cast<uint32_t>(((1ull << (31 + a.page_shift)) + pkv.page_size - 1) / pkv.page_size);
+    a.few_rows = kFewRows;
     const bool q8 = pkv.kv_mode == B200Q_KV_Q8;
+    const long long most = static_cast<long long>(max_q_len < n_tokens ? max_q_len : n_tokens) * a.group;
+    rc = launch_attn_few(a, hd, dtype == B200Q_F32, q8, static_cast<int>(std::min<long long>(most, kFewRows)), max_kv_len, st);
+    if (rc != B200Q_OK || most <= kFewRows) return rc;
     const dim3 grid(n_tokens, (heads + 3) / 4);
     auto go = [&](auto kern) { kern<<<grid, 128, 0, st>>>(a); };
     if (hd == 128) {

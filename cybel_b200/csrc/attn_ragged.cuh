@@ -1,0 +1,158 @@
+// Shared by the two kernels of b200q_attention_paged: the arguments, which
+// positions a row sees, and how raw products become exponents.
+#pragma once
+
+#include "ragged.cuh"
+
+namespace b200q {
+
+struct AttnArgs {
+    RaggedView r;
+    PagedView kv;
+    const void* q;
+    void* out;
+    const float* slopes;  // [heads] or NULL
+    const int* prefix;    // [batch] or NULL
+    long long q_stride, out_stride;
+    int heads;
+    int group;            // query heads per kv head
+    int window;           // 0: none
+    float scale, cap;     // cap 0: none
+    uint32_t page_mul;    // position / page = umulhi(2 position, page_mul) >> page_shift
+    int page_shift;
+    int few_rows;         // sequences with at most this many rows x group are the few-row kernel's
+    int row_blocks;       // few-row kernel: blocks of rows per sequence and kv head
+};
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr uint32_t kNoRow = 0xFFFFFFFFu;
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// cap * tanh(x / cap). fp16 rows: 1 - 2 / (e^2z + 1) from two approximate
+// instructions, off by about cap 2^-22 absolutely, which moves a softmax
+// weight by as much relatively (fp16 rounds it by 2^-12); fp32 rows: tanhf.
+template <bool PREC>
+__device__ __forceinline__ float capped(float x, float cap, float inv_cap) {
+    if constexpr (PREC) return cap * tanhf(x * inv_cap);
+    const float e = ex2(x * (2.0f * kLog2e * inv_cap));
+    return cap - 2.0f * cap * rcp_fast(e + 1.0f);
+}
+
+// The smallest power of two above x (finite, >= 0), at least 2^-126.
+__device__ __forceinline__ float pow2_above(float x) {
+    const int e = min((__float_as_int(x) & 0x7f800000) + 0x00800000, 0x7f000000);
+    return __int_as_float(e);
+}
+
+// What the rows of one tile of a sequence see: positions [0, pre) and, for
+// the row at position i, [i - window + 1, i]; n positions in all.
+struct Sight {
+    int n, pre, window;
+    // First position of the range that the row at position i sees by itself.
+    __device__ __forceinline__ int first(int i) const { return window > 0 ? max(0, i - window + 1) : 0; }
+    __device__ __forceinline__ bool sees(int i, int j) const { return j < pre || (j <= i && j >= first(i)); }
+    // Whether every row at lo .. hi sees all of j0 .. j1.
+    __device__ __forceinline__ bool all(int lo, int hi, int j0, int j1) const {
+        return j1 < pre || (j1 <= lo && j0 >= first(hi));
+    }
+};
+
+__device__ __forceinline__ Sight sight_of(const AttnArgs& a, int b) {
+    Sight s;
+    s.n = a.r.kv_len[b];
+    s.pre = a.prefix ? min(max(a.prefix[b], 0), max(s.n, 0)) : 0;
+    s.window = a.window;
+    return s;
+}
+
+// The tiles of T positions that rows at lo .. hi (lo <= hi, hi >= 0) need, in
+// order: those of the prefix before the rows' own range, then that range.
+template <int T>
+struct TileList {
+    int before, from, count;
+    __device__ __forceinline__ TileList(const Sight& s, int lo, int hi) {
+        from = s.first(max(lo, 0)) / T;
+        before = min((s.pre + T - 1) / T, from);
+        const int last = max(hi, s.pre - 1);
+        count = last < 0 ? 0 : before + last / T - from + 1;
+    }
+    __device__ __forceinline__ int at(int i) const { return (i < before ? i : from + i - before) * T; }
+};
+
+// Pool row of position j of sequence b, kv head h; kNoRow without one.
+__device__ __forceinline__ uint32_t row_of(const AttnArgs& a, int b, int h, int j) {
+    const int pg = static_cast<int>(__umulhi(2u * static_cast<uint32_t>(j), a.page_mul) >> a.page_shift);
+    const int slot = page_slot(a.kv, b, pg);
+    if (slot < 0) {
+        if (slot == -2) flag_bad_page(a.kv);
+        return kNoRow;
+    }
+    return static_cast<uint32_t>(pool_row(a.kv, slot, h, j - pg * a.kv.page));
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool valid) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(valid ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// ---- clusters ----------------------------------------------------------------
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Address of this CTA's shared address `a` in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t peer_addr(uint32_t a, uint32_t rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float4 ld_peer4(uint32_t a) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(a)
+                 : "memory");
+    return v;
+}
+__device__ __forceinline__ float2 ld_peer2(uint32_t a) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
+    return v;
+}
+
+__device__ __forceinline__ void store_out4(float* p, float4 v) { *reinterpret_cast<float4*>(p) = v; }
+__device__ __forceinline__ void store_out4(__half* p, float4 v) {
+    const __half2 a = __floats2half2_rn(v.x, v.y), b = __floats2half2_rn(v.z, v.w);
+    *reinterpret_cast<uint2*>(p) =
+        make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+
+int launch_attn_few(const AttnArgs& a, int hd, bool fp32, bool q8, int max_rows, int max_kv, cudaStream_t st);
+
+}  // namespace b200q

@@ -412,7 +412,9 @@ int check_paged(const PagedKV& p, int hd) {
         p.page_size <= 0 || p.pages_per_seq <= 0 || p.n_kv <= 0 || (q8 && (!p.k_scales || !p.v_scales)))
         return B200Q_EINVAL;
     if (hd != 64 && hd != 128) return B200Q_ESHAPE;
+    // positions and pool rows are 32-bit numbers in the kernels
     if (static_cast<long long>(p.pages_per_seq) * p.page_size > (1 << 30)) return B200Q_ESHAPE;
+    if (static_cast<long long>(p.n_slots) * p.n_kv > 0xFFFFFFFEll / p.page_size) return B200Q_ESHAPE;
     if (!aligned_to(p.k_pages, 16) || !aligned_to(p.v_pages, 16) || !aligned_to(p.page_table, 4) ||
         (q8 && (!aligned_to(p.k_scales, 4) || !aligned_to(p.v_scales, 4))))
         return B200Q_EALIGN;
