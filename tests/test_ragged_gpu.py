@@ -15,7 +15,13 @@ Tolerances, per element, fixed before the kernels ran:
   2^-11 for weights rounded to fp16 and 2^-11 for the output (2^-10 in all),
   2^-14 for exponentials and 32-bit sums; fp32 rows (weights in two fp16
   parts, 2^-22) 2^-19 in all; and 2^-24 absolute for fp16 outputs below the
-  smallest normal.
+  smallest normal. Weights in fp16 have a smallest step, too, which matters
+  where all but tiny weights meet exact zeros: the largest weight of a row is
+  kept at 2^10 or more, so a weight is rounded to a multiple of 2^-24 / 2^10 of
+  it, off by 2^-35; with Q8 scales the step is that of weight x scale / E,
+  E at most twice the largest scale, so a value term is off by at most
+  2^-35 x 2 max|v|. The softmax's sum is at least the largest weight, hence
+  n 2^-34 max|v| over n visible positions.
 """
 
 from __future__ import annotations
@@ -198,6 +204,7 @@ def _check_attend(c, layer, batch, q, got, scale=None, cap=0.0, slopes=None, win
                 qn[at:at + m], k, v, np.arange(n - m, n), n, scale, cap, None if slopes is None else slopes,
                 window, 0 if prefix is None else prefix[b], here)
             tol = bound + spread * (2.0 ** -10 + 2.0 ** -14 if f16 else 2.0 ** -19) + (2.0 ** -24 if f16 else 1e-30)
+            tol = tol + n * 2.0 ** -34 * np.abs(v[here], where=np.isfinite(v[here]), out=np.zeros_like(v[here])).max(initial=0)
             d = np.abs(got[at:at + m] - want)
             bad = ~(d <= tol)
             assert not bad.any(), (b, np.argwhere(bad)[:4], float(np.nanmax(d / tol)), int(bad.sum()), bad.size)
