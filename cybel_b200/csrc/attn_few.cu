@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) b200q_attn_few_kernel(const At
     for (int i = 0; i < NR; ++i) {
         const int r = r0 + g + 8 * i;
         const bool have = r < rows;
-        const int tok = have ? r / a.group : 0, head = kvh * a.group + (have ? r - tok * a.group : 0);
+        const int tok = have ? div_by(r, a.group_mul, a.group_shift) : 0, head = kvh * a.group + (have ? r - tok * a.group : 0);
         pos[i] = p0 + tok;
         slope[i] = a.slopes ? a.slopes[head] * kLog2e : 0.0f;
         const T* q = static_cast<const T*>(a.q) + (rr.x + tok) * a.q_stride + head * D;
@@ -301,11 +301,20 @@ __global__ void __launch_bounds__(kWarps * 32, 2) b200q_attn_few_kernel(const At
 #pragma unroll
         for (int i2 = 0; i2 < NR; ++i2) {
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                x[i2][v] *= mult[i2];
-                if (shaped) {
+            for (int v = 0; v < 4; ++v) x[i2][v] *= mult[i2];
+            if (shaped) {
+                if (a.cap > 0.0f) {
+#pragma unroll
+                    for (int v = 0; v < 4; v += 2) {
+                        const float2 z = mul2(make_float2(x[i2][v], x[i2][v + 1]), both(inv_cap));
+                        const float2 near = tanh_near(z);
+                        x[i2][v] = a.cap * (fabsf(z.x) > 1.0f ? tanh_far(z.x) : near.x);
+                        x[i2][v + 1] = a.cap * (fabsf(z.y) > 1.0f ? tanh_far(z.y) : near.y);
+                    }
+                }
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
                     const int j = j0 + 8 * (v >> 1) + 2 * c + (v & 1);
-                    if (a.cap > 0.0f) x[i2][v] = capped<PREC>(x[i2][v], a.cap, inv_cap);
                     x[i2][v] = x[i2][v] * kLog2e - slope[i2] * fabsf(static_cast<float>(pos[i2] - j));
                 }
             }
@@ -499,7 +508,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) b200q_attn_few_kernel(const At
         const int row = r0 + r;
         if (r >= nr) return;
         const float inv = lsum > 0.0f || lsum != lsum ? 1.0f / lsum : 0.0f;
-        const int tok = row / a.group, head = kvh * a.group + row - tok * a.group;
+        const int tok = div_by(row, a.group_mul, a.group_shift), head = kvh * a.group + row - tok * a.group;
         T* out = static_cast<T*>(a.out) + (rr.x + tok) * a.out_stride + head * D + e;
         store_out4(out, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
     };

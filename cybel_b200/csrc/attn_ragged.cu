@@ -59,8 +59,13 @@ int launch_attention_paged(const void* q, int dtype, int n_tokens, int batch, co
     a.scale = scale;
     a.cap = softcap;
     a.group = heads / pkv.n_kv;
-    while ((1ll << a.page_shift) < pkv.page_size) ++a.page_shift;
-    a.page_mul = static_cast<uint32_t>(((1ull << (31 + a.page_shift)) + pkv.page_size - 1) / pkv.page_size);
+    auto divisor = [](int d, uint32_t& mul, int& shift) {  // div_by
+        shift = 0;
+        while ((1ll << shift) < d) ++shift;
+        mul = static_cast<uint32_t>(((1ull << (31 + shift)) + d - 1) / d);
+    };
+    divisor(pkv.page_size, a.page_mul, a.page_shift);
+    divisor(a.group, a.group_mul, a.group_shift);
     a.few_rows = kFewRows;
     const bool q8 = pkv.kv_mode == B200Q_KV_Q8;
     const long long most = static_cast<long long>(max_q_len < n_tokens ? max_q_len : n_tokens) * a.group;

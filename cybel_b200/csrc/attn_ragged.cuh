@@ -18,14 +18,23 @@ struct AttnArgs {
     int group;            // query heads per kv head
     int window;           // 0: none
     float scale, cap;     // cap 0: none
-    uint32_t page_mul;    // position / page = umulhi(2 position, page_mul) >> page_shift
+    uint32_t page_mul;    // position / page = div_by(position, page_mul, page_shift)
     int page_shift;
+    uint32_t group_mul;   // the same of row / group
+    int group_shift;
     int few_rows;         // sequences with at most this many rows x group are the few-row kernel's
     int row_blocks;       // few-row kernel: blocks of rows per sequence and kv head
 };
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr uint32_t kNoRow = 0xFFFFFFFFu;
+
+// x / d for 0 <= x < 2^31: umulhi(2 x, mul) >> shift, shift = ceil(log2 d), mul
+// = ceil(2^(31 + shift) / d) (its excess e < d adds less than x e / (d
+// 2^(31 + shift)) < 1 / d to the quotient).
+__device__ __forceinline__ int div_by(int x, uint32_t mul, int shift) {
+    return static_cast<int>(__umulhi(2u * static_cast<uint32_t>(x), mul) >> shift);
+}
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -38,14 +47,46 @@ __device__ __forceinline__ float rcp_fast(float x) {
     return y;
 }
 
-// cap * tanh(x / cap). fp16 rows: 1 - 2 / (e^2z + 1) from two approximate
-// instructions, off by about cap 2^-22 absolutely, which moves a softmax
-// weight by as much relatively (fp16 rounds it by 2^-12); fp32 rows: tanhf.
-template <bool PREC>
-__device__ __forceinline__ float capped(float x, float cap, float inv_cap) {
-    if constexpr (PREC) return cap * tanhf(x * inv_cap);
-    const float e = ex2(x * (2.0f * kLog2e * inv_cap));
-    return cap - 2.0f * cap * rcp_fast(e + 1.0f);
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<uint64_t&>(d))
+        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<uint64_t&>(d))
+        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<uint64_t&>(d))
+        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+    return d;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+// tanh(z) for |z| <= 1: z P(z^2), P of degree 6 (minimax in the relative
+// error, by Remez's exchange: 2^-24).
+__device__ __forceinline__ float2 tanh_near(float2 z) {
+    const float2 u = mul2(z, z);
+    float2 p = fma2(u, both(1.041022634e-03f), both(-6.203379105e-03f));
+    p = fma2(p, u, both(2.028998042e-02f));
+    p = fma2(p, u, both(-5.345702957e-02f));
+    p = fma2(p, u, both(1.332520408e-01f));
+    p = fma2(p, u, both(-3.333283915e-01f));
+    p = fma2(p, u, both(9.999999502e-01f));
+    return mul2(p, z);
+}
+// tanh(z) as 1 - 2 / (e^2z + 1) from two approximate instructions: off by 2^-22
+// absolutely, which beyond 1 is as good as exact.
+__device__ __forceinline__ float tanh_far(float z) {
+    return 1.0f - 2.0f * rcp_fast(ex2(z * (2.0f * kLog2e)) + 1.0f);
 }
 
 // The smallest power of two above x (finite, >= 0), at least 2^-126.
@@ -91,7 +132,7 @@ struct TileList {
 
 // Pool row of position j of sequence b, kv head h; kNoRow without one.
 __device__ __forceinline__ uint32_t row_of(const AttnArgs& a, int b, int h, int j) {
-    const int pg = static_cast<int>(__umulhi(2u * static_cast<uint32_t>(j), a.page_mul) >> a.page_shift);
+    const int pg = div_by(j, a.page_mul, a.page_shift);
     const int slot = page_slot(a.kv, b, pg);
     if (slot < 0) {
         if (slot == -2) flag_bad_page(a.kv);

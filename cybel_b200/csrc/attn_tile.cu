@@ -16,14 +16,22 @@
 //    slots (128-byte swizzle, keys K-major, values MN-major as they lie).
 //    Thread r looks up row r's page one step ahead; fp16 rows come by
 //    cp.async, Q8 rows through registers, converted to their integer codes;
-//  * warp 12: issues the MMAs.
+//  * warps 12, 13: issue the MMAs of tile 0, 1 (one warp for both took 4850
+//    clocks a step, issuing one tile's while the other's were due).
 //
 // fp32 rows: q and the weights are each two fp16 parts (22 bits), both
-// products run twice into the same accumulators. Q8 scales multiply scores
-// and weights, the latter relative to a power of two above the scales so far.
+// products run twice into the same accumulators; Q8 scales multiply scores and
+// weights in fp32, the latter relative to a power of two above the scales so
+// far. fp16 rows take Q8 keys and values as code x scale rounded to fp16, which
+// is what their own type carries (2^-12 of a key's element moves a score by
+// 2^-12 / sqrt(head) of its size at random, an output by less than its own
+// rounding) and spares the softmax warps two products per score, half as much
+// again as all they do otherwise.
 // The output is rescaled in tensor memory by the softmax warps themselves and
-// only when a row's maximum rose by 2^kRise since the last time: by then the
-// product before is complete, because the barrier of S covers it.
+// only when a row's maximum rose by 2^kRise since the last time: the product
+// before is complete by then, because the barrier of S covers it. The weights
+// are handed over in two halves, so that the product starts under the second
+// half's exponentials.
 //
 // With few blocks of rows the positions are split over the CTAs of a cluster,
 // which join their outputs through shared memory at the end (as in
@@ -46,17 +54,21 @@ constexpr int kTiles = 2;
 constexpr int kCtaRows = kTiles * kRows;
 constexpr int kMaxCluster = 8;
 constexpr int kBadWords = 64;    // steps whose values were cleaned, one bit each
-constexpr float kRise = 5.0f;    // weights are at most 2^(kRise + kLift) = 2^15 in fp16
+// Weights are 2^(score - reference maximum + kLift); the reference follows a
+// row's maximum once that has risen by kRise, so they stay below 2^15 in fp16.
+constexpr float kRise = 5.0f;
 constexpr float kLift = 10.0f;
-// Registers per thread after the split; 128 x (2 x 176 + 104 + 56) = 65536 =
-// 512 x 128, what the block is launched with.
-constexpr int kSoftmaxRegs = 176, kLoaderRegs = 104, kIssuerRegs = 56;
+// Registers per thread after the split: 2 x softmax + loader + issuer = 512 =
+// 4 x 128, what the block is launched with. (Q8 loaders hold a step's codes.)
+constexpr int softmax_regs(bool q8) { return q8 ? 176 : 184; }
+constexpr int loader_regs(bool q8) { return q8 ? 96 : 72; }
+constexpr int issuer_regs(bool q8) { return 512 - 2 * softmax_regs(q8) - loader_regs(q8); }
 
-template <bool Q8>
+template <bool SCALES>
 struct Meta {
     uint32_t valid[4];           // bit: the position has a row that was loaded
-    float vmax[4];               // Q8: largest finite value scale of each warp's 32
-    float ks[kRows], vs[kRows];  // Q8
+    float vmax[4];               // largest finite value scale of each warp's 32
+    float ks[kRows], vs[kRows];
 };
 template <>
 struct Meta<false> {
@@ -71,11 +83,8 @@ struct Job {
     int rows;       // of the sequence
     int first_tok;  // batch row of the sequence's first token
     int p0;         // its position
+    Sight sight;
     int lo[kTiles], hi[kTiles];  // positions of the tiles' first and last rows (hi -1: no rows)
-    __device__ __forceinline__ bool needs(const Sight& s, int t, int j0) const {
-        const int top = max(hi[t], s.pre - 1);
-        return hi[t] >= max(lo[t], 0) && j0 <= top && (j0 < s.pre || j0 + kRows > s.first(max(lo[t], 0)));
-    }
     // Whether a value that is not finite has to be kept out of the product
     // over positions j0 .. : some row does not see all of them, or the rows'
     // weights have low parts, which turn an infinity into NaN.
@@ -85,6 +94,19 @@ struct Job {
     }
 };
 
+// Which of a CTA's steps a tile takes part in: those of the prefix, and
+// those that overlap what its own rows reach.
+struct Steps {
+    int prefix, from, to;
+    __device__ __forceinline__ Steps(const Sight& s, const TileList<kRows>& list, int i0, int lo, int hi) {
+        const bool any = hi >= max(lo, 0);
+        prefix = any ? (s.pre + kRows - 1) / kRows - i0 : 0;
+        from = list.before + max(s.first(max(lo, 0)) / kRows - list.from, 0) - i0;
+        to = any ? list.before + max(hi, s.pre - 1) / kRows - list.from - i0 : -1;
+    }
+    __device__ __forceinline__ bool has(int i) const { return i < prefix || (i >= from && i <= to); }
+};
+
 template <int D, bool PREC, bool Q8>
 struct Tile {
     static constexpr int kHalf = kRows * 128;               // 128 rows x 64 fp16
@@ -92,21 +114,22 @@ struct Tile {
     static constexpr int kParts = PREC ? 2 : 1;
     static constexpr int kQ = kTiles * kParts * kMat;
     static constexpr int kMeta = PREC ? 2 : 4;              // steps of per-position data in flight
-    static constexpr int kMetaBytes = kMeta * static_cast<int>(sizeof(Meta<Q8>));
-    static constexpr int kRest = kMetaBytes + 256 + kBadWords * 4 + 128;
+    static constexpr int kMetaBytes = kMeta * static_cast<int>(sizeof(Meta<PREC && Q8>));
+    static constexpr int kBarBytes = 320;
+    static constexpr int kRest = kMetaBytes + kBarBytes + kBadWords * 4 + 128;
     static constexpr int kFree = (227 * 1024 - kQ - kRest) / kMat;
     static constexpr int NS = kFree > 6 ? 6 : kFree;        // ring slots
     static constexpr int kRing = kQ;
     static constexpr int kMetaAt = kRing + NS * kMat;
     static constexpr int kBars = kMetaAt + kMetaBytes;
-    static constexpr int kBad = kBars + 256;
+    static constexpr int kBad = kBars + kBarBytes;
     static constexpr int kJob = kBad + kBadWords * 4;
     static constexpr int kTotal = kJob + 128;
     // after the loop, over Q and the ring: the tiles' outputs, then max and sum per row
     static constexpr int kMl = kTiles * kRows * D * 4;
-    static constexpr int kNumBars = 2 * NS + 2 * kMeta + 3 * kTiles + 1;
-    static_assert(NS >= 3 && kTotal <= 227 * 1024 && kMl + kCtaRows * 8 <= kMetaAt && kNumBars * 8 <= 256 &&
-                      sizeof(Job) + 8 <= 128,
+    static constexpr int kNumBars = 2 * NS + 2 * kMeta + 4 * kTiles + 1 + 4 * kTiles;
+    static_assert(NS >= 3 && kTotal <= 227 * 1024 && kMl + kCtaRows * 8 <= kMetaAt && kNumBars * 8 <= kBarBytes &&
+                      sizeof(Job) <= 116,
                   "shared memory");
 };
 
@@ -159,6 +182,21 @@ __device__ __forceinline__ uint32_t pack2(float x, float y) {
 }
 __device__ __forceinline__ float2 unpack2(uint32_t h) { return __half22float2(*reinterpret_cast<const __half2*>(&h)); }
 
+// The n lowest bits.
+__device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : (n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u); }
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float4 lds_f4(uint32_t a) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ void put2(float* p, float2 v) { p[0] = v.x, p[1] = v.y; }
+
 // Byte address of 16-byte chunk c (of D / 8) of row r of an operand tile.
 template <int HALF>
 __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
@@ -185,10 +223,12 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
     using T = typename std::conditional<PREC, float, __half>::type;
     constexpr int NS = S::NS;
     constexpr int kMeta = S::kMeta;
+    constexpr bool SC = PREC && Q8;  // scales beside the codes; fp16 rows get them multiplied in
     extern __shared__ __align__(1024) uint8_t smem[];
     Job* job_s = reinterpret_cast<Job*>(smem + S::kJob);
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + S::kJob + 120);
     volatile uint32_t* dead = reinterpret_cast<volatile uint32_t*>(smem + S::kJob + 124);
+    volatile uint32_t* any_bad = reinterpret_cast<volatile uint32_t*>(smem + S::kJob + 116);  // any of bad_bits
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t C = cluster_size(), rank = cluster_rank();
     griddep_launch_dependents();
@@ -212,6 +252,7 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
         if (lane == 0) {
             job_s->live = x >= 0;
             *dead = 0;
+            *any_bad = 0;
         }
         for (int b0 = 0; b0 < a.r.batch && x >= 0; b0 += 32) {
             const int mine = blocks(b0 + lane);
@@ -230,7 +271,8 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
                 j.rows = (rr.y - rr.x) * a.group;
                 j.row0 = (x - (upto - mine)) * kCtaRows;
                 j.first_tok = rr.x;
-                j.p0 = a.r.kv_len[j.b] - (rr.y - rr.x);
+                j.sight = sight_of(a, j.b);
+                j.p0 = j.sight.n - (rr.y - rr.x);
                 for (int t = 0; t < kTiles; ++t) {
                     const int r0 = j.row0 + t * kRows, r1 = min(r0 + kRows, j.rows) - 1;
                     j.lo[t] = j.p0 + r0 / a.group;
@@ -252,12 +294,13 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
     auto mempty = [&](int i) { return bar0 + 8u * (2 * NS + kMeta + i % kMeta); };
     auto qfull = [&](int t) { return bar0 + 8u * (2 * NS + 2 * kMeta + t); };
     auto sready = [&](int t) { return bar0 + 8u * (2 * NS + 2 * kMeta + kTiles + t); };
-    auto pready = [&](int t) { return bar0 + 8u * (2 * NS + 2 * kMeta + 2 * kTiles + t); };
-    const uint32_t done = bar0 + 8u * (2 * NS + 2 * kMeta + 3 * kTiles);
+    auto pready = [&](int t, int half) { return bar0 + 8u * (2 * NS + 2 * kMeta + 2 * kTiles + 2 * t + half); };
+    const uint32_t done = bar0 + 8u * (2 * NS + 2 * kMeta + 4 * kTiles);
+    auto turn = [&](int t, int w) { return done + 8u * (1 + 4 * t + w); };
     if (threadIdx.x == 32) {
         for (int i = 0; i < NS; ++i) {
-            mbar_init(kvfull(i), kRows);
-            mbar_init(kvempty(i), 1);
+            mbar_init(kvfull(i), 4);
+            mbar_init(kvempty(i), kTiles);
         }
         for (int i = 0; i < kMeta; ++i) {
             mbar_init(mfull(i), 4);
@@ -266,9 +309,11 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
         for (int t = 0; t < kTiles; ++t) {
             mbar_init(qfull(t), kRows);
             mbar_init(sready(t), 1);
-            mbar_init(pready(t), 4);
+            mbar_init(pready(t, 0), 4);
+            mbar_init(pready(t, 1), 4);
+            for (int w = 0; w < 4; ++w) mbar_init(turn(t, w), 1);
         }
-        mbar_init(done, 1);
+        mbar_init(done, kTiles);
         fence_mbar_init();
     }
     __syncthreads();
@@ -282,7 +327,7 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
     tc_fence_after();
     const uint32_t tmem = *tmem_holder;
     const Job& job = *job_s;
-    const Sight sight = sight_of(a, job.b);
+    const Sight sight = job.sight;
     const int lo = job.lo[0], hi = max(job.hi[0], job.hi[1]);
     const TileList<kRows> list(sight, lo, hi);
     const int n_all = hi < 0 ? 0 : list.count;
@@ -290,76 +335,71 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
     const int n = static_cast<int>(static_cast<long long>(n_all) * (rank + 1) / C) - i0;  // steps of this CTA
     const Waiter wait{dead, a.kv.status};
     const uint32_t sbase = smem_addr(smem);
-    Meta<Q8>* meta = reinterpret_cast<Meta<Q8>*>(smem + S::kMetaAt);
+    Meta<SC>* meta = reinterpret_cast<Meta<SC>*>(smem + S::kMetaAt);
     uint32_t* bad_bits = reinterpret_cast<uint32_t*>(smem + S::kBad);
     auto pos_of = [&](int i) { return list.at(i0 + i); };
     float2* ml = reinterpret_cast<float2*>(smem + S::kMl);
     constexpr uint32_t kO = 256;  // tensor-memory columns: S (then P) of the tiles, then their outputs
 
     if (warp >= 12) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssuerRegs));
-        if (warp == 12) {
-            // ---------------- MMA issuer ----------------
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(issuer_regs(Q8)));
+        if (warp < 12 + kTiles) {
+            // ---------------- MMA issuer of tile t ----------------
             constexpr uint32_t idS = idesc_of(kRows, false), idO = idesc_of(D, true);
-            bool ok = true;
-            int np[kTiles] = {0, 0};  // steps of each tile so far
-            for (int s = 0; s <= n && ok; ++s) {
-                for (int t = 0; t < kTiles && ok; ++t) {
-                    if (s > 0 && job.needs(sight, t, pos_of(s - 1))) {
-                        const int item = 2 * (s - 1) + 1;
-                        ok = wait(pready(t), (np[t] - 1) & 1) && wait(kvfull(item), (item / NS) & 1);
-                        ok = __all_sync(0xffffffffu, ok);
-                        if (!ok) break;
-                        tc_fence_after();
-                        const uint32_t d = tmem + kO + t * D, p = tmem + t * kRows;
-                        const uint64_t v = desc_sw128(sbase + S::kRing + (item % NS) * S::kMat, S::kHalf);
-                        if (elect_one()) {
+            const int t = warp - 12;
+            const Steps steps(sight, list, i0, job.lo[t], job.hi[t]);
+            const uint32_t ts = tmem + t * kRows, to = tmem + kO + t * D;
+            const uint64_t q0 = desc_sw128(sbase + t * S::kParts * S::kMat, 0);
+            const uint64_t k0 = desc_sw128(sbase + S::kRing, 0), v0 = desc_sw128(sbase + S::kRing, S::kHalf);
+            // One thread throughout, and the waits for operands that are early before
+            // the wait for the weights, so that nothing stands between those and the
+            // products (a wait by the whole warp costs 150 clocks even when it is over).
+            if (elect_one()) {
+                bool ok = wait(qfull(t), 0);
+                int np = 0;  // steps so far
+                for (int s = 0; s <= n && ok; ++s) {
+                    const int ki = 2 * s, vi = 2 * s - 1;
+                    const bool pv = s > 0 && steps.has(s - 1), qk = s < n && steps.has(s);
+                    ok = (s == n || wait(kvfull(ki), (ki / NS) & 1)) && (s == 0 || wait(kvfull(vi), (vi / NS) & 1));
+                    if (pv) {
+                        const uint64_t v = v0 + ((vi % NS) * (S::kMat >> 4));
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            ok = ok && wait(pready(t, half), (np - 1) & 1);
+                            if (!ok) break;
+                            tc_fence_after();
 #pragma unroll
                             for (int part = 0; part < S::kParts; ++part)
 #pragma unroll
-                                for (int k = 0; k < kRows / 16; ++k)
-                                    tc_mma_f16_ts(d, p + part * 64 + k * 8, v + k * (2048 >> 4), idO,
-                                                  np[t] > 1 || part > 0 || k > 0 ? 1u : 0u);
+                                for (int k = 4 * half; k < 4 * half + 4; ++k)
+                                    tc_mma_f16_ts(to, ts + part * 64 + k * 8, v + k * (2048 >> 4), idO,
+                                                  np > 1 || part > 0 || k > 0 ? 1u : 0u);
                         }
-                        __syncwarp();
                     }
-                    if (s < n && job.needs(sight, t, pos_of(s))) {
-                        const int item = 2 * s;
-                        if (np[t] == 0) ok = wait(qfull(t), 0);
-                        ok = ok && wait(kvfull(item), (item / NS) & 1);
-                        ok = __all_sync(0xffffffffu, ok);
-                        if (!ok) break;
+                    if (!ok) break;
+                    if (qk) {
                         tc_fence_after();
-                        const uint32_t d = tmem + t * kRows;
-                        const uint64_t k0 = desc_sw128(sbase + S::kRing + (item % NS) * S::kMat, 0);
-                        const uint64_t q0 = desc_sw128(sbase + t * S::kParts * S::kMat, 0);
-                        if (elect_one()) {
+                        const uint64_t kk = k0 + ((ki % NS) * (S::kMat >> 4));
 #pragma unroll
-                            for (int part = 0; part < S::kParts; ++part)
+                        for (int part = 0; part < S::kParts; ++part)
 #pragma unroll
-                                for (int k = 0; k < D / 16; ++k) {
-                                    const uint32_t off = ((k >> 2) * S::kHalf + (k & 3) * 32) >> 4;
-                                    tc_mma_f16(d, q0 + ((part * S::kMat) >> 4) + off, k0 + off, idS,
-                                               part > 0 || k > 0 ? 1u : 0u);
-                                }
-                            tc_commit(sready(t));
-                        }
-                        __syncwarp();
-                        ++np[t];
+                            for (int k = 0; k < D / 16; ++k) {
+                                const uint32_t off = ((k >> 2) * S::kHalf + (k & 3) * 32) >> 4;
+                                tc_mma_f16(ts, q0 + ((part * S::kMat) >> 4) + off, kk + off, idS,
+                                           part > 0 || k > 0 ? 1u : 0u);
+                            }
+                        tc_commit(sready(t));
+                        ++np;
                     }
+                    if (s > 0) tc_commit(kvempty(vi));
+                    if (s < n) tc_commit(kvempty(ki));
                 }
-                if (ok && elect_one()) {
-                    if (s > 0) tc_commit(kvempty(2 * (s - 1) + 1));
-                    if (s < n) tc_commit(kvempty(2 * s));
-                    if (s == n) tc_commit(done);
-                }
-                __syncwarp();
+                tc_commit(done);  // what was issued still has to finish
             }
-            if (!ok && elect_one()) tc_commit(done);  // what was issued still has to finish
             __syncwarp();
         }
     } else if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoaderRegs));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(loader_regs(Q8)));
         // ---------------- loader ----------------
         const int r = threadIdx.x - 256, w = warp - 8;
         const int hi_seen = max(hi, sight.pre - 1), lo_seen = sight.first(max(lo, 0));
@@ -368,20 +408,28 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
             const int j = pos_of(i) + r;
             return (j <= hi_seen && (j < sight.pre || j >= lo_seen)) ? row_of(a, job.b, job.kvh, j) : kNoRow;
         };
+        float ks_next = 0.0f, vs_next = 0.0f;  // Q8: the scales of the row looked up last
+        auto scales_of = [&](uint32_t row) {
+            if constexpr (Q8) {
+                ks_next = row != kNoRow ? __ldg(a.kv.ks + row) : 0.0f;
+                vs_next = row != kNoRow ? __ldg(a.kv.vs + row) : 0.0f;
+            }
+        };
         auto put_meta = [&](int i, uint32_t row) {
-            Meta<Q8>& m = meta[i % kMeta];
+            Meta<SC>& m = meta[i % kMeta];
             const uint32_t bits = __ballot_sync(0xffffffffu, row != kNoRow);
             if (lane == 0) m.valid[w] = bits;
             if constexpr (Q8) {
-                float ks = 0.0f, vs = 0.0f;
-                if (row != kNoRow) ks = a.kv.ks[row], vs = a.kv.vs[row];
-                if (!(fabsf(vs) < INFINITY) && job.template mixed<PREC>(sight, pos_of(i))) {
-                    vs = 0.0f;
+                if (!(fabsf(vs_next) < INFINITY) && job.template mixed<PREC>(sight, pos_of(i))) {
+                    vs_next = 0.0f;
                     atomicOr(bad_bits + (i >> 5) % kBadWords, 1u << (i & 31));
+                    *any_bad = 1;
                 }
-                m.ks[r] = ks;
-                m.vs[r] = vs;
-                const float mx = fabsf(vs) < INFINITY ? fabsf(vs) : 0.0f;
+            }
+            if constexpr (SC) {
+                m.ks[r] = ks_next;
+                m.vs[r] = vs_next;
+                const float mx = fabsf(vs_next) < INFINITY ? fabsf(vs_next) : 0.0f;
                 const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(mx));
                 if (lane == 0) m.vmax[w] = __uint_as_float(top);
             }
@@ -409,41 +457,66 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
                             sts128(at, u);
                         }
                     }
-                    if (bad) atomicOr(bad_bits + (x >> 6) % kBadWords, 1u << ((x >> 1) & 31));
+                    if (bad) {
+                        atomicOr(bad_bits + (x >> 6) % kBadWords, 1u << ((x >> 1) & 31));
+                        *any_bad = 1;
+                    }
                 }
                 fence_proxy_async_smem();
-                mbar_arrive(kvfull(x));
+                __syncwarp();
+                if (lane == 0) mbar_arrive(kvfull(x));
             };
+            // Shared offsets of this thread's copies within the warp's 32 rows: they
+            // repeat every 8 rows, up to the rows themselves.
+            int handed = 0;  // items finished
+            constexpr int PAT = 8 / RPI;
+            uint32_t pat[PAT];
+#pragma unroll
+            for (int t = 0; t < PAT; ++t) pat[t] = chunk_at<S::kHalf>(w * 32 + t * RPI + lane / CH, lane % CH);
             for (int i = 0; i < n && ok; ++i) {
                 const uint32_t row = ahead;
                 ahead = look(i + 1);
                 ok = __all_sync(0xffffffffu, wait(mempty(i), ((i / kMeta) & 1) ^ 1));
                 if (!ok) break;
                 put_meta(i, row);
+                // The warp's 32 rows one after the other in one page, as nearly always?
+                const uint32_t row0 = __shfl_sync(0xffffffffu, row, 0);
+                const bool run = __all_sync(0xffffffffu, row != kNoRow && row == row0 + lane);
                 for (int part = 0; part < 2; ++part) {
                     const int x = 2 * i + part;
-                    ok = __all_sync(0xffffffffu, wait(kvempty(x), ((x / NS) & 1) ^ 1));
-                    if (!ok) break;
+                    if (!__all_sync(0xffffffffu, mbar_test_wait(kvempty(x), ((x / NS) & 1) ^ 1))) {
+                        // the ring is full: hand over what is on its way first
+                        cp_async_wait<0>();
+                        while (handed < x) finish(handed++);
+                        ok = __all_sync(0xffffffffu, wait(kvempty(x), ((x / NS) & 1) ^ 1));
+                        if (!ok) break;
+                    }
                     const uint32_t slot = sbase + S::kRing + (x % NS) * S::kMat;
                     const uint8_t* src = static_cast<const uint8_t*>(part ? a.kv.v : a.kv.k) + (lane % CH) * 16;
+                    if (run) {
+                        src += static_cast<long long>(row0 + lane / CH) * (2 * D);
 #pragma unroll
-                    for (int t = 0; t < NI; ++t) {
-                        const int rl = t * RPI + lane / CH;
-                        const uint32_t rw = __shfl_sync(0xffffffffu, row, rl);
-                        const bool have = rw != kNoRow;
-                        cp_async16(slot + chunk_at<S::kHalf>(w * 32 + rl, lane % CH),
-                                   src + (have ? static_cast<long long>(rw) * (2 * D) : 0), have);
+                        for (int t = 0; t < NI; ++t)
+                            cp_async16(slot + pat[t % PAT] + (t / PAT) * 1024, src + t * (RPI * 2 * D), true);
+                    } else {
+#pragma unroll 4
+                        for (int t = 0; t < NI; ++t) {
+                            const uint32_t rw = __shfl_sync(0xffffffffu, row, t * RPI + lane / CH);
+                            const bool have = rw != kNoRow;
+                            cp_async16(slot + chunk_at<S::kHalf>(w * 32 + t * RPI + lane / CH, lane % CH),
+                                       src + (have ? static_cast<long long>(rw) * (2 * D) : 0), have);
+                        }
                     }
                     cp_async_commit();
-                    if (x >= LA) {
+                    if (handed <= x - LA) {
                         cp_async_wait<LA>();
-                        finish(x - LA);
+                        finish(handed++);
                     }
                 }
             }
             cp_async_wait<0>();
             if (ok)
-                for (int x = max(0, 2 * n - LA); x < 2 * n; ++x) finish(x);
+                while (handed < 2 * n) finish(handed++);
         } else {
             constexpr int CH = D / 16, RPI = 32 / CH, NI = 32 / RPI;
             uint4 kreg[NI], vreg[NI];
@@ -458,26 +531,47 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
                                        lane % CH);
                 }
             };
-            auto put = [&](const uint4 (&reg)[NI], int x) {
+            auto put = [&](const uint4 (&reg)[NI], int x, uint32_t scale) {
                 const uint32_t slot = sbase + S::kRing + (x % NS) * S::kMat;
 #pragma unroll
                 for (int t = 0; t < NI; ++t) {
                     const int row = w * 32 + t * RPI + lane / CH, c = 2 * (lane % CH);
                     const uint32_t u[4] = {reg[t].x ^ 0x80808080u, reg[t].y ^ 0x80808080u, reg[t].z ^ 0x80808080u,
                                            reg[t].w ^ 0x80808080u};
-                    sts128(slot + chunk_at<S::kHalf>(row, c),
-                           make_uint4(codes_fp16(u[0], 0x4140), codes_fp16(u[0], 0x4342), codes_fp16(u[1], 0x4140),
-                                      codes_fp16(u[1], 0x4342)));
-                    sts128(slot + chunk_at<S::kHalf>(row, c + 1),
-                           make_uint4(codes_fp16(u[2], 0x4140), codes_fp16(u[2], 0x4342), codes_fp16(u[3], 0x4140),
-                                      codes_fp16(u[3], 0x4342)));
+                    uint32_t h[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) h[k] = codes_fp16(u[k >> 1], (k & 1) ? 0x4342 : 0x4140);
+                    if constexpr (!PREC) {
+                        // code x scale rounded once to fp16: the scale as two parts
+                        const uint32_t sc = __shfl_sync(0xffffffffu, scale, t * RPI + lane / CH);
+                        const __half2 s2 = *reinterpret_cast<const __half2*>(&sc);
+                        const __half2 hi = __low2half2(s2), lo = __high2half2(s2);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const __half2 cd = *reinterpret_cast<const __half2*>(&h[k]);
+                            const __half2 v = __hfma2(cd, hi, __hmul2(cd, lo));
+                            h[k] = *reinterpret_cast<const uint32_t*>(&v);
+                        }
+                    }
+                    sts128(slot + chunk_at<S::kHalf>(row, c), make_uint4(h[0], h[1], h[2], h[3]));
+                    sts128(slot + chunk_at<S::kHalf>(row, c + 1), make_uint4(h[4], h[5], h[6], h[7]));
                 }
                 fence_proxy_async_smem();
-                mbar_arrive(kvfull(x));
+                __syncwarp();
+                if (lane == 0) mbar_arrive(kvfull(x));
+            };
+            // A scale as fp16 parts hi | lo, 22 bits of it (the low part of one that is
+            // not finite would be NaN: it is left out).
+            auto split = [](float sc) {
+                const __half hi = __float2half_rn(sc);
+                const float rest = sc - __half2float(hi);
+                const __half lo = __float2half_rn(fabsf(rest) < INFINITY ? rest : 0.0f);
+                return static_cast<uint32_t>(__half_as_ushort(hi)) | (static_cast<uint32_t>(__half_as_ushort(lo)) << 16);
             };
             uint32_t row = ahead;
             ahead = look(1);
             if (n > 0) {
+                scales_of(row);
                 fetch(kreg, a.kv.k, row);
                 fetch(vreg, a.kv.v, row);
             }
@@ -485,68 +579,88 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
                 ok = __all_sync(0xffffffffu, wait(mempty(i), ((i / kMeta) & 1) ^ 1));
                 if (!ok) break;
                 put_meta(i, row);
+                const uint32_t ks2 = split(ks_next), vs2 = split(vs_next);
                 row = ahead;
+                scales_of(row);
                 ahead = look(i + 2);
                 ok = __all_sync(0xffffffffu, wait(kvempty(2 * i), ((2 * i / NS) & 1) ^ 1));
                 if (!ok) break;
-                put(kreg, 2 * i);
+                put(kreg, 2 * i, ks2);
                 fetch(kreg, a.kv.k, row);
                 ok = __all_sync(0xffffffffu, wait(kvempty(2 * i + 1), (((2 * i + 1) / NS) & 1) ^ 1));
                 if (!ok) break;
-                put(vreg, 2 * i + 1);
+                put(vreg, 2 * i + 1, vs2);
                 fetch(vreg, a.kv.v, row);
             }
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(softmax_regs(Q8)));
         // ---------------- softmax of tile t, row tid ----------------
         const int t = warp >> 2, tid = threadIdx.x & 127;
         const int row = job.row0 + t * kRows + tid;
         const bool have = row < job.rows;
-        const int tok = have ? row / a.group : 0, head = job.kvh * a.group + (have ? row - tok * a.group : 0);
+        const int tok = have ? div_by(row, a.group_mul, a.group_shift) : 0, head = job.kvh * a.group + (have ? row - tok * a.group : 0);
         const int pos = job.p0 + tok;
         const float slope = a.slopes ? a.slopes[head] * kLog2e : 0.0f;
         float mult = a.scale;
         {
-            // Q: this row, fp16 as it is, fp32 as two parts of q 2^10 / E
-            const T* q = static_cast<const T*>(a.q) + (job.first_tok + tok) * a.q_stride + head * D;
+            // Q of the warp's 32 rows, a row (fp32) or two (fp16) per load: fp16 as it
+            // is, fp32 as two parts of q 2^10 / E, E a power of two above the row
             const uint32_t dst = sbase + t * S::kParts * S::kMat;
+            const int w32 = (warp & 3) * 32, first_row = job.row0 + t * kRows + w32;
+            auto source = [&](int r) {  // row first_row + r, NULL past the sequence
+                const int rw = first_row + r;
+                const int tk = div_by(rw, a.group_mul, a.group_shift);
+                return rw < job.rows ? static_cast<const T*>(a.q) + (job.first_tok + tk) * a.q_stride +
+                                           (job.kvh * a.group + rw - tk * a.group) * D
+                                     : nullptr;
+            };
             if constexpr (!PREC) {
-#pragma unroll 4
-                for (int c = 0; c < D / 8; ++c)
-                    sts128(dst + chunk_at<S::kHalf>(tid, c),
-                           have ? *(reinterpret_cast<const uint4*>(q) + c) : make_uint4(0u, 0u, 0u, 0u));
-            } else {
-                float amax = 0.0f;
-                if (have)
-#pragma unroll 8
-                    for (int c = 0; c < D / 4; ++c) {
-                        const float4 v = *(reinterpret_cast<const float4*>(q) + c);
-                        amax = fmaxf(amax, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
-                    }
-                const float E = fmaxf(pow2_above(amax < INFINITY ? amax : 0.0f), 7.8886090522e-31f);  // 2^-100
-                const float down = __fdiv_rn(1024.0f, E);
-                mult *= E * 0.0009765625f;
-#pragma unroll 2
-                for (int c = 0; c < D / 8; ++c) {
-                    uint4 h = make_uint4(0u, 0u, 0u, 0u), l = h;
-                    if (have) {
-                        const float4 x = *(reinterpret_cast<const float4*>(q) + 2 * c);
-                        const float4 y = *(reinterpret_cast<const float4*>(q) + 2 * c + 1);
-                        const float v[8] = {x.x * down, x.y * down, x.z * down, x.w * down,
-                                            y.x * down, y.y * down, y.z * down, y.w * down};
-                        uint32_t hh[4], ll[4];
+                constexpr int CH = D / 8, RPI = 32 / CH, NI = 32 / RPI;
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            hh[k] = pack2(v[2 * k], v[2 * k + 1]);
-                            const float2 f = unpack2(hh[k]);
-                            ll[k] = pack2(v[2 * k] - f.x, v[2 * k + 1] - f.y);
-                        }
-                        h = make_uint4(hh[0], hh[1], hh[2], hh[3]);
-                        l = make_uint4(ll[0], ll[1], ll[2], ll[3]);
+                for (int k = 0; k < NI; ++k) {
+                    const int r = k * RPI + lane / CH;
+                    const T* src = source(r);
+                    cp_async16(dst + chunk_at<S::kHalf>(w32 + r, lane % CH),
+                               src ? src + (lane % CH) * 8 : static_cast<const T*>(a.q), src != nullptr);
+                }
+                cp_async_commit();
+                cp_async_wait<0>();
+            } else {
+                constexpr int CH = D / 4, RPI = 32 / CH, NI = 32 / RPI, NB = 8;  // float4 per row; rows in flight
+#pragma unroll 1
+                for (int k0 = 0; k0 < NI; k0 += NB) {
+                    float4 v[NB];
+#pragma unroll
+                    for (int k = 0; k < NB; ++k) {
+                        const T* src = source((k0 + k) * RPI + lane / CH);
+                        v[k] = src ? *reinterpret_cast<const float4*>(src + (lane % CH) * 4)
+                                   : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                     }
-                    sts128(dst + chunk_at<S::kHalf>(tid, c), h);
-                    sts128(dst + S::kMat + chunk_at<S::kHalf>(tid, c), l);
+#pragma unroll
+                    for (int k = 0; k < NB; ++k) {
+                        const int r = (k0 + k) * RPI + lane / CH;
+                        float amax = fmaxf(fmaxf(fabsf(v[k].x), fabsf(v[k].y)), fmaxf(fabsf(v[k].z), fabsf(v[k].w)));
+#pragma unroll
+                        for (int o = CH / 2; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+                        const float E = fmaxf(pow2_above(amax < INFINITY ? amax : 0.0f), 7.8886090522e-31f);  // 2^-100
+                        const float down = __fdiv_rn(1024.0f, E);
+#pragma unroll
+                        for (int h = 0; h < RPI; ++h) {
+                            const float Eh = __shfl_sync(0xffffffffu, E, h * CH);
+                            if (lane == (k0 + k) * RPI + h) mult = a.scale * (Eh * 0.0009765625f);
+                        }
+                        const float2 x = make_float2(v[k].x * down, v[k].y * down);
+                        const float2 y = make_float2(v[k].z * down, v[k].w * down);
+                        const uint32_t h0 = pack2(x.x, x.y), h1 = pack2(y.x, y.y);
+                        const float2 f0 = unpack2(h0), f1 = unpack2(h1);
+                        const uint32_t l0 = pack2(x.x - f0.x, x.y - f0.y), l1 = pack2(y.x - f1.x, y.y - f1.y);
+                        const uint32_t at =
+                            dst + chunk_at<S::kHalf>(w32 + r, (lane % CH) >> 1) + ((lane & 1) << 3);
+                        asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(h0), "r"(h1) : "memory");
+                        asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at + S::kMat), "r"(l0), "r"(l1)
+                                     : "memory");
+                    }
                 }
             }
             fence_proxy_async_smem();
@@ -557,133 +671,185 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
         const float to_log2 = shaped ? 1.0f : mult * kLog2e;  // factor left for the exponent
         const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
         const uint32_t ts = tmem + lanes + t * kRows, to = tmem + lanes + kO + t * D;
+        const Steps mine(sight, list, i0, job.lo[t], job.hi[t]);
+        const int t_lo = job.lo[t], t_hi = job.hi[t];
         float m = -INFINITY, l = 0.0f;
-        float E = 0.0f, inv_E = 0.0f;
+        float E = 0.0f, log_E = 0.0f;  // SC: weights, their sum and the output are relative to E
         int steps = 0;
         bool ok = true;
         for (int i = 0; i < n && ok; ++i) {
-            const int j0 = pos_of(i);
             ok = __all_sync(0xffffffffu, wait(mfull(i), (i / kMeta) & 1));
             if (!ok) break;
-            const Meta<Q8>& md = meta[i % kMeta];
-            if (!job.needs(sight, t, j0)) {
-                __syncwarp();
-                if (lane == 0) mbar_arrive(mempty(i));
+            const Meta<SC>& md = meta[i % kMeta];
+            // The exponentials' turn: the two warps that share a scheduler take
+            // theirs one after the other, tile 0's first, so that one tile's
+            // products run under the other's exponentials (left to themselves both
+            // tiles fell in step and each unit idled half the time).
+            const uint32_t my_turn = turn(t, warp & 3), next_turn = turn(t ^ 1, warp & 3);
+            const bool wait_turn = t == 1 || i > 0;
+            if (!mine.has(i)) {
+                ok = __all_sync(0xffffffffu, !wait_turn || wait(my_turn, (i - 1 + t) & 1));
+                if (lane == 0) {
+                    mbar_arrive(next_turn);
+                    mbar_arrive(mempty(i));
+                }
                 continue;
+            }
+            // Positions of the step that the row sees, 32 to a word: below the
+            // prefix, or from a0 to a1.
+            const int j0 = pos_of(i);
+            const uint4 valid = *reinterpret_cast<const uint4*>(md.valid);
+            const bool whole = (valid.x & valid.y & valid.z & valid.w) == 0xFFFFFFFFu &&
+                               sight.all(t_lo, t_hi, j0, j0 + kRows - 1);
+            uint32_t see[4] = {valid.x, valid.y, valid.z, valid.w};
+            if (!whole) {
+                const int pre = sight.pre - j0, a0 = sight.first(pos) - j0, a1 = pos - j0;
+#pragma unroll
+                for (int w = 0; w < 4; ++w)
+                    see[w] &= below(pre - 32 * w) | (below(a1 + 1 - 32 * w) & ~below(a0 - 32 * w));
+            }
+            float unit = 1.0f;
+            if constexpr (SC) {
+                const float4 vm = *reinterpret_cast<const float4*>(md.vmax);
+                const float mx = fmaxf(fmaxf(vm.x, vm.y), fmaxf(vm.z, vm.w));
+                if (mx >= E) {
+                    const float e2 = fmaxf(pow2_above(mx), 8.6736173799e-19f);  // 2^-60
+                    unit = E / e2;  // powers of two; 0 at the first step
+                    E = e2;
+                    log_E = static_cast<float>((__float_as_int(E) >> 23) - 127);
+                }
             }
             ok = __all_sync(0xffffffffu, wait(sready(t), steps & 1));
             if (!ok) break;
             tc_fence_after();
+
+            uint32_t ks_at = 0, vs_at = 0;
+            if constexpr (SC) ks_at = smem_addr(md.ks), vs_at = smem_addr(md.vs);
+            // ---- the step's exponents (times to_log2, plus row_off), from S
             float x[kRows];
+            float row_off = 0.0f;
 #pragma unroll
             for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, x + 32 * c);
             tmem_wait_ld();
 #pragma unroll
             for (int c = 0; c < 4; ++c) tmem_loaded32(x + 32 * c);
-            const uint4 valid = *reinterpret_cast<const uint4*>(md.valid);
-            const bool whole = (valid.x & valid.y & valid.z & valid.w) == 0xFFFFFFFFu &&
-                               sight.all(job.lo[t], job.hi[t], j0, j0 + kRows - 1);
-            if constexpr (Q8) {
+            if constexpr (SC) {
 #pragma unroll
                 for (int c = 0; c < kRows; c += 4) {
-                    const float4 k = *reinterpret_cast<const float4*>(md.ks + c);
-                    x[c] *= k.x, x[c + 1] *= k.y, x[c + 2] *= k.z, x[c + 3] *= k.w;
+                    const float4 k = lds_f4(ks_at + c * 4);
+                    put2(x + c, mul2(make_float2(x[c], x[c + 1]), make_float2(k.x, k.y)));
+                    put2(x + c + 2, mul2(make_float2(x[c + 2], x[c + 3]), make_float2(k.z, k.w)));
                 }
             }
             if (shaped) {
+                const float f1 = a.cap > 0.0f ? mult * inv_cap : mult * kLog2e;
+#pragma unroll
+                for (int c = 0; c < kRows; c += 2) put2(x + c, mul2(make_float2(x[c], x[c + 1]), both(f1)));
                 if (a.cap > 0.0f) {
+                    float far[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (int c = 0; c < kRows; ++c) x[c] = capped<PREC>(x[c] * mult, a.cap, inv_cap) * kLog2e;
-                } else {
+                    for (int c = 0; c < kRows; c += 8)
 #pragma unroll
-                    for (int c = 0; c < kRows; ++c) x[c] *= mult * kLog2e;
+                        for (int u = 0; u < 4; ++u)
+                            far[u] = max3(far[u], fabsf(x[c + 2 * u]), fabsf(x[c + 2 * u + 1]));
+                    const float f2 = a.cap * kLog2e;
+                    if (__any_sync(0xffffffffu, fmaxf(fmaxf(far[0], far[1]), fmaxf(far[2], far[3])) > 1.0f)) {
+#pragma unroll
+                        for (int c = 0; c < kRows; ++c) x[c] = f2 * tanh_far(x[c]);
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < kRows; c += 2)
+                            put2(x + c, mul2(tanh_near(make_float2(x[c], x[c + 1])), both(f2)));
+                    }
                 }
                 if (a.slopes) {
                     const float d0 = static_cast<float>(pos - j0);
+                    if (j0 + kRows - 1 <= t_lo) {  // all behind the rows: the distance is d0 - c
+                        row_off = -slope * d0;
 #pragma unroll
-                    for (int c = 0; c < kRows; ++c) x[c] -= slope * fabsf(d0 - static_cast<float>(c));
+                        for (int c = 0; c < kRows; c += 2)
+                            put2(x + c, fma2(both(slope), make_float2(c, c + 1), make_float2(x[c], x[c + 1])));
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < kRows; ++c) x[c] = fmaf(-slope, fabsf(d0 - static_cast<float>(c)), x[c]);
+                    }
                 }
             }
             if (!whole) {
-                // positions of the step that the row sees: below `pre`, or from `a0` to `a1`
-                const int pre = sight.pre - j0, a0 = sight.first(pos) - j0, a1 = pos - j0;
-                const uint32_t vw[4] = {valid.x, valid.y, valid.z, valid.w};
 #pragma unroll
-                for (int c = 0; c < kRows; ++c) {
-                    const bool see = ((vw[c >> 5] >> (c & 31)) & 1u) && (c < pre || (c >= a0 && c <= a1));
-                    if (!see) x[c] = -INFINITY;
-                }
+                for (int c = 0; c < kRows; ++c)
+                    if (!(see[c >> 5] & (1u << (c & 31)))) x[c] = -INFINITY;
             }
-            float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            // ---- the reference maximum
+            {
+                float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int c = 0; c < kRows; c += 8)
+                for (int c = 0; c < kRows; c += 8)
 #pragma unroll
-                for (int u = 0; u < 4; ++u) tops[u] = fmaxf(tops[u], fmaxf(x[c + 2 * u], x[c + 2 * u + 1]));
-            const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * to_log2;
-            float unit = 1.0f;
-            if constexpr (Q8) {
-                const float4 vm = *reinterpret_cast<const float4*>(md.vmax);
-                const float mx = fmaxf(fmaxf(vm.x, vm.y), fmaxf(vm.z, vm.w));
-                if (mx >= E) {
-                    const float e2 = pow2_above(mx);
-                    unit = E / e2;  // powers of two; 0 at the first step
-                    E = e2;
-                    inv_E = 1.0f / E;
-                }
-            }
-            const bool rise = top > m + kRise;
-            if (__any_sync(0xffffffffu, rise) || unit != 1.0f) {
-                const float mn = rise ? top : m;
-                const float f = m == -INFINITY ? 1.0f : ex2(m - mn);
-                m = mn;
-                l *= f;
-                if (steps > 0) {
-                    const float fu = f * unit;
+                    for (int u = 0; u < 4; ++u) tops[u] = max3(tops[u], x[c + 2 * u], x[c + 2 * u + 1]);
+                const float top = fmaf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])), to_log2, row_off);
+                const bool rise = top > m + kRise;
+                if (__any_sync(0xffffffffu, rise || unit != 1.0f)) {
+                    const float mn = rise ? top : m;
+                    const float f = (m == -INFINITY ? 1.0f : ex2(m - mn)) * (steps > 0 ? unit : 1.0f);
+                    m = mn;
+                    l *= f;
+                    if (steps > 0) {
 #pragma unroll
-                    for (int c = 0; c < D; c += 16) {
-                        float o[16];
-                        tmem_ld16(to + c, o);
-                        tmem_wait_ld();
-                        tmem_loaded16(o);
+                        for (int c = 0; c < D; c += 16) {
+                            float o[16];
+                            tmem_ld16(to + c, o);
+                            tmem_wait_ld();
+                            tmem_loaded16(o);
 #pragma unroll
-                        for (int k = 0; k < 16; ++k) o[k] *= fu;
-                        tmem_st16(to + c, o);
+                            for (int k = 0; k < 16; ++k) o[k] *= f;
+                            tmem_st16(to + c, o);
+                        }
                     }
                 }
             }
-            const float base = m == -INFINITY ? 0.0f : kLift - m;
-            float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            ok = __all_sync(0xffffffffu, !wait_turn || wait(my_turn, (i - 1 + t) & 1));
+            if (!ok) break;
+            // ---- weights, a quarter of the positions at a time
+            const float base = m == -INFINITY ? 0.0f : kLift - m - log_E + row_off;
+            float2 s2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                uint32_t hi32[32], lo32[32];
+            for (int quarter = 0; quarter < 4; ++quarter) {
+                uint32_t hi16[16], lo16[16];
+                float4 v4;
 #pragma unroll
-                for (int c = 0; c < 64; c += 4) {
-                    float p[4];
-                    float4 v = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
-                    if constexpr (Q8) v = *reinterpret_cast<const float4*>(md.vs + half * 64 + c);
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        p[u] = ex2(fmaf(x[half * 64 + c + u], to_log2, base));
-                        sums[u] += p[u];
+                for (int c = 0; c < 32; c += 2) {
+                    const float* xq = x + quarter * 32 + c;
+                    if constexpr (SC) {
+                        if (c % 4 == 0) v4 = lds_f4(vs_at + (quarter * 32 + c) * 4);
                     }
-                    if constexpr (Q8) p[0] *= v.x * inv_E, p[1] *= v.y * inv_E, p[2] *= v.z * inv_E, p[3] *= v.w * inv_E;
-                    hi32[c / 2] = pack2(p[0], p[1]);
-                    hi32[c / 2 + 1] = pack2(p[2], p[3]);
+                    const float2 u = fma2(make_float2(xq[0], xq[1]), both(to_log2), both(base));
+                    float2 p = make_float2(ex2(u.x), ex2(u.y));
+                    s2[(c >> 1) & 1] = add2(s2[(c >> 1) & 1], p);
+                    if constexpr (SC) p = mul2(p, c % 4 == 0 ? make_float2(v4.x, v4.y) : make_float2(v4.z, v4.w));
+                    hi16[c / 2] = pack2(p.x, p.y);
                     if constexpr (PREC) {
-                        const float2 h0 = unpack2(hi32[c / 2]), h1 = unpack2(hi32[c / 2 + 1]);
-                        lo32[c / 2] = pack2(p[0] - h0.x, p[1] - h0.y);
-                        lo32[c / 2 + 1] = pack2(p[2] - h1.x, p[3] - h1.y);
+                        const float2 h = unpack2(hi16[c / 2]);
+                        lo16[c / 2] = pack2(p.x - h.x, p.y - h.y);
                     }
                 }
-                tmem_st32(ts + half * 32, hi32);
-                if constexpr (PREC) tmem_st32(ts + 64 + half * 32, lo32);
+                if (quarter == 2) {  // the first half has arrived in tensor memory long ago
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(pready(t, 0));
+                }
+                tmem_st16(ts + quarter * 16, hi16);
+                if constexpr (PREC) tmem_st16(ts + 64 + quarter * 16, lo16);
             }
-            l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+            if (lane == 0) mbar_arrive(next_turn);
+            const float2 st = add2(s2[0], s2[1]);
+            l += st.x + st.y;
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
-                mbar_arrive(pready(t));
+                mbar_arrive(pready(t, 1));
                 mbar_arrive(mempty(i));
             }
             ++steps;
@@ -692,13 +858,16 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
         ok = __all_sync(0xffffffffu, wait(done, 0));
         tc_fence_after();
         const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-        const float fin = C == 1 ? (Q8 ? inv * E : inv) : (Q8 ? E : 1.0f);
-        if (C > 1) ml[t * kRows + tid] = make_float2(m, l);
-        bool bad = false;
-        for (int k = 0; k < kBadWords; ++k) bad |= bad_bits[k] != 0;
-        T* out = static_cast<T*>(a.out) + (job.first_tok + tok) * a.out_stride + head * D;
-        // The other tile's products may still read the ring: its outputs go
-        // over Q and the ring only once both are done (`done` covers all).
+        const float fin = C == 1 ? inv : (SC && l > 0.0f ? E : 1.0f);
+        if (C > 1) ml[t * kRows + tid] = make_float2(m, l * fin);
+        const bool bad = *any_bad != 0;
+        // Through shared memory, so that rows leave in one piece: fp16 or fp32 rows
+        // over the tile's Q (C = 1, this warp's rows only), or the fp32 parts of the
+        // cluster over Q and the ring. `done` covers both tiles' products. 16-byte
+        // chunks are spread by the row, so that a warp's rows fall on all banks.
+        constexpr int kRowBytes = D * static_cast<int>(sizeof(T));
+        const uint32_t stage = C == 1 ? sbase + t * S::kParts * S::kMat + tid * kRowBytes
+                                      : sbase + (t * kRows + tid) * (D * 4);
 #pragma unroll 1
         for (int c = 0; c < D; c += 32) {
             float o[32];
@@ -732,19 +901,32 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
                     }
                 }
             }
-            if (C == 1) {
-                if (have) {
-#pragma unroll
-                    for (int k = 0; k < 32; k += 4)
-                        store_out4(out + c + k, make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]));
-                }
-            } else {
-                // chunk (of 4 floats) spread by the row, so that a warp's rows fall on all banks
+            if (PREC || C > 1) {
 #pragma unroll
                 for (int k = 0; k < 32; k += 4)
-                    sts128(sbase + (t * kRows + tid) * (D * 4) + ((((c + k) >> 2) ^ (tid & 7)) << 4),
+                    sts128(stage + ((((c + k) >> 2) ^ (tid & 7)) << 4),
                            make_uint4(__float_as_uint(o[k]), __float_as_uint(o[k + 1]), __float_as_uint(o[k + 2]),
                                       __float_as_uint(o[k + 3])));
+            } else {
+#pragma unroll
+                for (int k = 0; k < 32; k += 8)
+                    sts128(stage + ((((c + k) >> 3) ^ (tid & 7)) << 4),
+                           make_uint4(pack2(o[k], o[k + 1]), pack2(o[k + 2], o[k + 3]), pack2(o[k + 4], o[k + 5]),
+                                      pack2(o[k + 6], o[k + 7])));
+            }
+        }
+        if (C == 1) {
+            __syncwarp();
+            constexpr int CH = kRowBytes / 16, RPI = 32 / CH, NI = 32 / RPI;
+            const int w32 = (warp & 3) * 32;
+#pragma unroll 8
+            for (int k = 0; k < NI; ++k) {
+                const int r = w32 + k * RPI + lane / CH, rw = job.row0 + t * kRows + r;
+                if (rw >= job.rows) continue;
+                const uint4 v = lds128(sbase + t * S::kParts * S::kMat + r * kRowBytes + (((lane % CH) ^ (r & 7)) << 4));
+                const int tk = div_by(rw, a.group_mul, a.group_shift);
+                *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (job.first_tok + tk) * a.out_stride +
+                                          (job.kvh * a.group + rw - tk * a.group) * D + (lane % CH) * (16 / sizeof(T))) = v;
             }
         }
         tc_fence_before();
@@ -782,7 +964,7 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
             acc.x += v[k].x * f, acc.y += v[k].y * f, acc.z += v[k].z * f, acc.w += v[k].w * f;
         }
         const float inv = L > 0.0f || L != L ? 1.0f / L : 0.0f;
-        const int tok = row / a.group, head = job.kvh * a.group + row - tok * a.group;
+        const int tok = div_by(row, a.group_mul, a.group_shift), head = job.kvh * a.group + row - tok * a.group;
         T* out = static_cast<T*>(a.out) + (job.first_tok + tok) * a.out_stride + head * D + 4 * e;
         store_out4(out, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
     }
