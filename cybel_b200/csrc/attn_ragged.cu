@@ -59,11 +59,6 @@ int launch_attention_paged(const void* q, int dtype, int n_tokens, int batch, co
     a.scale = scale;
     a.cap = softcap;
     a.group = heads / pkv.n_kv;
-    auto divisor = [](int d, uint32_t& mul, int& shift) {  // div_by
-        shift = 0;
-        while ((1ll << shift) < d) ++shift;
-        mul = static_cast<uint32_t>(((1ull << (31 + shift)) + d - 1) / d);
-    };
     divisor(pkv.page_size, a.page_mul, a.page_shift);
     divisor(a.group, a.group_mul, a.group_shift);
     a.few_rows = kFewRows;

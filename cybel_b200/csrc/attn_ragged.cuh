@@ -27,14 +27,6 @@ struct AttnArgs {
 };
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr uint32_t kNoRow = 0xFFFFFFFFu;
-
-// x / d for 0 <= x < 2^31: umulhi(2 x, mul) >> shift, shift = ceil(log2 d), mul
-// = ceil(2^(31 + shift) / d) (its excess e < d adds less than x e / (d
-// 2^(31 + shift)) < 1 / d to the quotient).
-__device__ __forceinline__ int div_by(int x, uint32_t mul, int shift) {
-    return static_cast<int>(__umulhi(2u * static_cast<uint32_t>(x), mul) >> shift);
-}
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -46,30 +38,6 @@ __device__ __forceinline__ float rcp_fast(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-
-// Two fp32 operations in one instruction.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;"
-        : "=l"(reinterpret_cast<uint64_t&>(d))
-        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
-    return d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    float2 d;
-    asm("add.rn.f32x2 %0, %1, %2;"
-        : "=l"(reinterpret_cast<uint64_t&>(d))
-        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
-    return d;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    float2 d;
-    asm("mul.rn.f32x2 %0, %1, %2;"
-        : "=l"(reinterpret_cast<uint64_t&>(d))
-        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
-    return d;
-}
-__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
 // tanh(z) for |z| <= 1: z P(z^2), P of degree 6 (minimax in the relative
 // error, by Remez's exchange: 2^-24).

@@ -15,6 +15,7 @@
 // 2^-24 relative).
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
 
 #include "internal.h"
 #include "ragged.cuh"
@@ -23,41 +24,72 @@ namespace b200q {
 
 namespace {
 
-constexpr int kRopeThreads = 256;
-constexpr int kMaxRot = 256;  // rotated elements of a head: one cos/sin pair per thread of two rows
+constexpr int kRopeThreads = 128;
+constexpr int kMaxRot = 256;    // rotated elements of a head
+constexpr int kMaxRows = 4;     // rows of one CTA
+// Units a thread loads before it stores the first (rotated rows: 62 / 53 / 58
+// us for 2 / 3 / 4 at 8191 x 64 heads), and the units of query heads that a
+// thread of an append takes one after the other (6 x 1000 tokens into Q8 pages:
+// 77 us for 4, 72 for 8, two of them in flight; 84 with four).
+constexpr int kRowsInFlight = 3, kAppendInFlight = 2, kHeadsPerThread = 8;
 
-// Rounded to the nearest fp16 / kept.
 template <typename T>
 __device__ __forceinline__ float load1(const T* p) {
     return static_cast<float>(*p);
 }
-__device__ __forceinline__ void store1(float* p, float v) { *p = v; }
-__device__ __forceinline__ void store1(__half* p, float v) { *p = __float2half_rn(v); }
 
-// N consecutive elements as floats; N * sizeof(T) is 8 or 16 and p aligned to it.
-template <int N>
-__device__ __forceinline__ void load_n(const float* p, float (&v)[N]) {
-    static_assert(N == 4, "one 16-byte load");
-    const float4 x = *reinterpret_cast<const float4*>(p);
-    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+// V consecutive elements of T as loaded, 16 bytes at a time (V = 4 or 8 fp32, 8
+// fp16), 8 bytes (4 fp16) or one element.
+template <typename T, int V>
+struct Vec {
+    static constexpr int W = sizeof(T) * V / 4;
+    uint32_t w[W];
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (W >= 4) {
+#pragma unroll
+            for (int k = 0; k < W; k += 4) {
+                const uint4 x = __ldcs(reinterpret_cast<const uint4*>(p) + k / 4);
+                w[k] = x.x, w[k + 1] = x.y, w[k + 2] = x.z, w[k + 3] = x.w;
+            }
+        } else {
+            const uint2 x = *reinterpret_cast<const uint2*>(p);
+            w[0] = x.x, w[1] = x.y;
+        }
+    }
+    __device__ __forceinline__ float get(int e) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[e]);
+        else return __half2float(__ushort_as_half(static_cast<unsigned short>(w[e >> 1] >> (16 * (e & 1)))));
+    }
+};
+template <typename T>
+struct Vec<T, 1> {
+    T x;
+    __device__ __forceinline__ void load(const T* p) { x = *p; }
+    __device__ __forceinline__ float get(int) const { return static_cast<float>(x); }
+};
+template <int V>
+__device__ __forceinline__ void store_v(float* p, const float (&v)[V]) {
+    if constexpr (V == 1) {
+        *p = v[0];
+    } else {
+#pragma unroll
+        for (int e = 0; e < V; e += 4) *reinterpret_cast<float4*>(p + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+    }
 }
-template <int N>
-__device__ __forceinline__ void load_n(const __half* p, float (&v)[N]) {
-    static_assert(N == 4, "one 8-byte load");
-    const uint2 x = *reinterpret_cast<const uint2*>(p);
-    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&x.x));
-    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&x.y));
-    v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
-}
-template <int N>
-__device__ __forceinline__ void store_n(float* p, const float (&v)[N]) {
-    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-}
-template <int N>
-__device__ __forceinline__ void store_n(__half* p, const float (&v)[N]) {
-    const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
-    *reinterpret_cast<uint2*>(p) =
-        make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+template <int V>
+__device__ __forceinline__ void store_v(__half* p, const float (&v)[V]) {
+    if constexpr (V == 1) {
+        *p = __float2half_rn(v[0]);
+    } else {
+        uint32_t w[V / 2];
+#pragma unroll
+        for (int e = 0; e < V / 2; ++e) {
+            const __half2 h = __floats2half2_rn(v[2 * e], v[2 * e + 1]);
+            w[e] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        if constexpr (V == 8) __stcs(reinterpret_cast<uint4*>(p), make_uint4(w[0], w[1], w[2], w[3]));
+        else *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    }
 }
 
 // cos and sin (times mag) of pos * turn, turn in 2^-64 turns.
@@ -71,73 +103,159 @@ __device__ __forceinline__ float2 cos_sin(int pos, uint64_t turn, float mag) {
     const float cc = (quarter & 1u) ? -s : c, ss = (quarter & 1u) ? c : s;
     return (quarter & 2u) ? make_float2(-cc * mag, -ss * mag) : make_float2(cc * mag, ss * mag);
 }
+// The same in fp64, by the Taylor series about 0: an eighth of a turn is
+// pi / 4 at most, where the first terms left out are below 2^-56 (sin: x^17 /
+// 17!, cos: x^18 / 18!).
 __device__ __forceinline__ double2 cos_sin64(int pos, uint64_t turn, double mag) {
     const uint64_t a = static_cast<uint64_t>(static_cast<uint32_t>(pos)) * turn;
     const uint64_t quarter = (a + (1ull << 61)) >> 62;
     const long long rest = static_cast<long long>(a - (quarter << 62));
-    double s, c;
-    sincospi(static_cast<double>(rest) * 1.0842021724855044e-19, &s, &c);  // 2^-63
+    const double x = static_cast<double>(rest) * (6.283185307179586476925 / 18446744073709551616.0);  // 2 pi 2^-64
+    const double u = -x * x;
+    double s = 1.0 / 1307674368000.0, c = 1.0 / 20922789888000.0;  // 1 / 15!, 1 / 16!
+    s = fma(s, u, 1.0 / 6227020800.0);
+    s = fma(s, u, 1.0 / 39916800.0);
+    s = fma(s, u, 1.0 / 362880.0);
+    s = fma(s, u, 1.0 / 5040.0);
+    s = fma(s, u, 1.0 / 120.0);
+    s = fma(s, u, 1.0 / 6.0);
+    s = fma(s * u, x, x);
+    c = fma(c, u, 1.0 / 87178291200.0);
+    c = fma(c, u, 1.0 / 479001600.0);
+    c = fma(c, u, 1.0 / 3628800.0);
+    c = fma(c, u, 1.0 / 40320.0);
+    c = fma(c, u, 1.0 / 720.0);
+    c = fma(c, u, 1.0 / 24.0);
+    c = fma(c, u, 0.5);
+    c = fma(c, u, 1.0);
     const double cc = (quarter & 1u) ? -s : c, ss = (quarter & 1u) ? c : s;
     return (quarter & 2u) ? make_double2(-cc * mag, -ss * mag) : make_double2(cc * mag, ss * mag);
 }
 
 // How one head's elements are cut into units that read and write the same
-// elements: a pair unit is one rotated pair (V = 1) or four elements of each
-// half of the pairs (V = 4, half layout) or four elements of two pairs (V = 4,
-// interleaved); a copy unit is the V elements after the rotated part.
+// elements: a pair unit is V elements of each half of the pairs (half layout)
+// or V elements of V / 2 pairs (interleaved); a copy unit the V elements after
+// the rotated part. V = 1: one pair, one element.
 struct RopeShape {
     int hd;
     int rot;
     int half;        // layout: pairs (p, p + rot / 2) instead of (2p, 2p + 1)
     int units;       // per head
     int pair_units;  // the first of them
+    uint32_t unit_mul;  // index / units = div_by
+    int unit_shift;
 };
 
-// y = R x for unit u of one head; cs: this row's [rot / 2] cos, sin.
-template <int V, typename T>
-__device__ __forceinline__ void rope_unit(const RopeShape& s, const float2* cs, const T* x, T* y, int u) {
-    if constexpr (V == 1) {
-        if (u < s.pair_units) {
-            const int i = s.half ? u : 2 * u, j = s.half ? u + s.rot / 2 : 2 * u + 1;
-            const float a = load1(x + i), b = load1(x + j);
-            store1(y + i, a * cs[u].x - b * cs[u].y);
-            store1(y + j, a * cs[u].y + b * cs[u].x);
-        } else {
-            const int i = s.rot + u - s.pair_units;
-            y[i] = x[i];
+// Rotates `heads` heads of one row by the threads of the CTA: src heads hd
+// elements apart, dst heads dst_step. A thread keeps to one unit and its
+// angles and walks the heads, kFlight of them loaded before the first is
+// stored. cs: cos, sin of the row's pairs (unused when nothing is rotated).
+// A copy unit goes the same way and keeps what it read.
+template <int V, int kFlight, typename T, typename TO>
+__device__ __forceinline__ void rotate_heads(const RopeShape& s, const float2* cs, const T* src, TO* dst,
+                                             long long dst_step, int heads) {
+    int u = threadIdx.x, h0 = 0, ustep = kRopeThreads, hstep = 1;
+    if (s.units <= kRopeThreads) {
+        h0 = div_by(threadIdx.x, s.unit_mul, s.unit_shift);
+        u = threadIdx.x - h0 * s.units;
+        ustep = s.units;
+        hstep = div_by(kRopeThreads, s.unit_mul, s.unit_shift);
+        if (h0 >= hstep) return;  // the remainder of the threads
+    }
+    for (; u < s.units; u += ustep) {
+        const bool turn = u < s.pair_units;
+        const bool two = turn && (s.half || V == 1);
+        const int p = two ? u * V : u * V / 2;
+        const int i = !turn ? s.rot + (u - s.pair_units) * V : (V == 1 && !s.half ? 2 * u : u * V);
+        const int j = i + (s.half ? s.rot / 2 : 1);
+        float c[V], n[V];  // per element of the first vector (half), or per pair (interleaved)
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const float2 t = turn && (two || e < V / 2) ? cs[p + e] : make_float2(1.0f, 0.0f);
+            c[e] = t.x, n[e] = t.y;
         }
-    } else {
-        float a[V], o[V];
-        if (u >= s.pair_units) {
-            const int i = s.rot + (u - s.pair_units) * V;
-            load_n<V>(x + i, a);
-            store_n<V>(y + i, a);
-        } else if (s.half) {
-            float b[V], o2[V];
-            const int i = u * V, j = i + s.rot / 2;
-            load_n<V>(x + i, a);
-            load_n<V>(x + j, b);
+#pragma unroll 1
+        for (int h = h0; h < heads; h += hstep * kFlight) {
+            Vec<T, V> a[kFlight], b[kFlight];
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const float2 t = cs[i + e];
-                o[e] = a[e] * t.x - b[e] * t.y;
-                o2[e] = a[e] * t.y + b[e] * t.x;
+            for (int k = 0; k < kFlight; ++k) {
+                const int hh = h + k * hstep;
+                if (hh >= heads) continue;
+                a[k].load(src + hh * s.hd + i);
+                if (two) b[k].load(src + hh * s.hd + j);
             }
-            store_n<V>(y + i, o);
-            store_n<V>(y + j, o2);
-        } else {
-            const int i = u * V;
-            load_n<V>(x + i, a);
 #pragma unroll
-            for (int e = 0; e < V; e += 2) {
-                const float2 t = cs[(i + e) / 2];
-                o[e] = a[e] * t.x - a[e + 1] * t.y;
-                o[e + 1] = a[e] * t.y + a[e + 1] * t.x;
+            for (int k = 0; k < kFlight; ++k) {
+                const int hh = h + k * hstep;
+                if (hh >= heads) continue;
+                TO* y = dst + hh * dst_step;
+                float o[V];
+                if (two) {
+                    float o2[V];
+#pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        const float2 r = fma2(both(b[k].get(e)), make_float2(-n[e], c[e]),
+                                              mul2(both(a[k].get(e)), make_float2(c[e], n[e])));
+                        o[e] = r.x, o2[e] = r.y;
+                    }
+                    store_v(y + j, o2);
+                } else if (V > 1 && turn) {
+#pragma unroll
+                    for (int e = 0; e + 1 < V; e += 2) {
+                        const float2 r = fma2(both(a[k].get(e + 1)), make_float2(-n[e / 2], c[e / 2]),
+                                              mul2(both(a[k].get(e)), make_float2(c[e / 2], n[e / 2])));
+                        o[e] = r.x, o[e + 1] = r.y;
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < V; ++e) o[e] = a[k].get(e);
+                }
+                store_v(y + i, o);
             }
-            store_n<V>(y + i, o);
         }
     }
 }
+
+// One unit of one head, loaded and stored apart, for threads that take units
+// of any head and row in turn.
+template <typename T, int V>
+struct RopeUnit {
+    Vec<T, V> a, b;
+    int i, p;       // first element; first pair, -1 for a copy
+    bool two;       // a second vector, rot / 2 elements on
+    __device__ __forceinline__ void load(const RopeShape& s, const T* x, int u) {
+        two = u < s.pair_units && (s.half || V == 1);
+        p = u >= s.pair_units ? -1 : (two ? u * V : u * V / 2);
+        i = u >= s.pair_units ? s.rot + (u - s.pair_units) * V : (V == 1 && !s.half ? 2 * u : u * V);
+        a.load(x + i);
+        if (two) b.load(x + i + (s.half ? s.rot / 2 : 1));
+    }
+    template <typename TO>
+    __device__ __forceinline__ void store(const RopeShape& s, const float2* cs, TO* y) const {
+        float o[V];
+        if (p < 0) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) o[e] = a.get(e);
+        } else if (two) {
+            float o2[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float2 t = cs[p + e];
+                o[e] = a.get(e) * t.x - b.get(e) * t.y;
+                o2[e] = a.get(e) * t.y + b.get(e) * t.x;
+            }
+            store_v(y + i + (s.half ? s.rot / 2 : 1), o2);
+        } else {
+#pragma unroll
+            for (int e = 0; e + 1 < V; e += 2) {
+                const float2 t = cs[p + e / 2];
+                o[e] = a.get(e) * t.x - a.get(e + 1) * t.y;
+                o[e + 1] = a.get(e) * t.y + a.get(e + 1) * t.x;
+            }
+        }
+        store_v(y + i, o);
+    }
+};
 
 struct RopeRowsArgs {
     const void* x;
@@ -150,27 +268,44 @@ struct RopeRowsArgs {
     RopeShape s;
 };
 
+// Bound by its bytes for prompts, by latency for a step: a thread's loads go
+// out before the angles are computed, which need positions from memory first.
 template <int V, typename T>
 __global__ void __launch_bounds__(kRopeThreads) b200q_rope_rows_kernel(const RopeRowsArgs a) {
-    __shared__ float2 cs[kRopeThreads];  // rows_per_cta x rot / 2
+    __shared__ float2 cs[kMaxRows * kMaxRot / 2];
     griddep_launch_dependents();
     griddep_wait();
     const int np = a.s.rot / 2;
-    const int r0 = blockIdx.x * a.rows_per_cta;
+    const int r0 = blockIdx.x * a.rows_per_cta, h0 = blockIdx.y * a.heads_per_cta;
     const int nr = min(a.rows_per_cta, a.rows - r0);
-    for (int i = threadIdx.x; i < nr * np; i += kRopeThreads)
-        cs[i] = cos_sin(a.pos[r0 + i / np], a.turns[i % np], a.mag);
-    __syncthreads();
-    const int h0 = blockIdx.y * a.heads_per_cta;
-    const int per_row = min(a.heads_per_cta, a.heads - h0) * a.s.units;
-    for (int r = 0; r < nr; ++r) {
-        const T* x = static_cast<const T*>(a.x) + (r0 + r) * a.x_stride + h0 * a.s.hd;
-        T* y = static_cast<T*>(a.y) + (r0 + r) * a.y_stride + h0 * a.s.hd;
-#pragma unroll 4
-        for (int i = threadIdx.x; i < per_row; i += kRopeThreads) {
-            const int h = i / a.s.units, u = i - h * a.s.units;
-            rope_unit<V>(a.s, cs + r * np, x + h * a.s.hd, y + h * a.s.hd, u);
+    const int per_row = min(a.heads_per_cta, a.heads - h0) * a.s.units, total = nr * per_row;
+    const T* x = static_cast<const T*>(a.x) + r0 * a.x_stride + h0 * a.s.hd;
+    T* y = static_cast<T*>(a.y) + r0 * a.y_stride + h0 * a.s.hd;
+    bool angles = false;
+    for (int i0 = threadIdx.x; i0 - static_cast<int>(threadIdx.x) < total; i0 += kRopeThreads * kRowsInFlight) {
+        RopeUnit<T, V> u[kRowsInFlight];
+        int at[kRowsInFlight], row[kRowsInFlight];  // head's first element, row (-1: none)
+#pragma unroll
+        for (int k = 0; k < kRowsInFlight; ++k) {
+            int i = i0 + k * kRopeThreads;
+            row[k] = -1;
+            if (i >= total) continue;
+            int r = 0;
+            while (i >= per_row) i -= per_row, ++r;
+            const int h = div_by(i, a.s.unit_mul, a.s.unit_shift);
+            row[k] = r;
+            at[k] = h * a.s.hd;
+            u[k].load(a.s, x + r * a.x_stride + at[k], i - h * a.s.units);
         }
+        if (!angles) {
+            for (int i = threadIdx.x; i < nr * np; i += kRopeThreads)
+                cs[i] = cos_sin(a.pos[r0 + i / np], a.turns[i % np], a.mag);
+            __syncthreads();
+            angles = true;
+        }
+#pragma unroll
+        for (int k = 0; k < kRowsInFlight; ++k)
+            if (row[k] >= 0) u[k].store(a.s, cs + row[k] * np, y + row[k] * a.y_stride + at[k]);
     }
 }
 
@@ -181,9 +316,14 @@ struct AppendArgs {
     void* q_out;             // NULL: no queries
     const uint64_t* turns;   // NULL: no rotation (s.rot == 0)
     long long q_stride, kv_stride, q_out_stride;
-    int heads, heads_per_cta;
+    int heads, rows_per_cta;
+    int ctas;                   // of a block of rows:
+    int kv_per_cta, kv_ctas;    // 0 .. kv_ctas - 1 take its kv heads
+    int heads_per_cta;          // and the others its query heads
+    bool walk;                  // query heads by rotate_heads, a row after the other
+    bool kv_wide;               // Q8: rows can be read eight elements at a time
     double mag;
-    RopeShape s;
+    RopeShape s, plain;         // with rotation (keys, queries) and without (values)
 };
 
 // The Q8 row quantizer of the paged store (model_graph.cpp:1545-1573), as the
@@ -191,102 +331,200 @@ struct AppendArgs {
 __device__ __forceinline__ float q8_scale(float amax) {
     return amax > 0.0f ? __fdiv_rn(amax, 127.0f) : __fdiv_rn(1.0f, 127.0f);
 }
-__device__ __forceinline__ int8_t q8_code(float x, float inv) {
-    const int c = static_cast<int>(roundf(__fmul_rn(x, inv)));
-    return static_cast<int8_t>(max(-127, min(127, c)));
+// round() of the definition (halves away from zero), as a byte: to the nearest
+// integer by adding 1.5 2^23, halves that went to the even side put right.
+__device__ __forceinline__ uint32_t q8_code(float x, float inv) {
+    const float y = fminf(fmaxf(__fmul_rn(x, inv), -127.0f), 127.0f);
+    const float t = __fadd_rn(y, 12582912.0f);
+    const float rest = __fsub_rn(y, __fsub_rn(t, 12582912.0f));  // exact
+    int c = __float_as_int(t);
+    if (rest == 0.5f && y > 0.0f) ++c;
+    if (rest == -0.5f && y < 0.0f) --c;
+    return static_cast<uint32_t>(c) & 0xFFu;
 }
 
-// One CTA per row of the batch and group of query heads; the first group also
-// writes the row's keys and values. Bound by the bytes of q (read and
-// written) for prompts and by latency for decode steps.
+// Position of batch row `row` and the sequence that holds it (-1: none), by a
+// warp: the entries of cu_q not above the row are counted 32 at a time, one
+// trip to memory instead of a search's log2(batch).
+__device__ __forceinline__ int2 locate(const RaggedView& r, int row, int lane) {
+    int count = 0;
+    for (int b0 = 0; b0 <= r.batch; b0 += 32)
+        count += __popc(__ballot_sync(0xffffffffu, b0 + lane <= r.batch && r.cu_q[min(b0 + lane, r.batch)] <= row));
+    const int b = count - 1;
+    if (b < 0 || b >= r.batch) return make_int2(0, -1);
+    return make_int2(r.kv_len[b] - (seq_rows(r, b).y - row), b);
+}
+
+// CTAs: for each block of rows_per_cta rows its kv heads, then its query heads
+// (side by side, so that the quantizer's long chains run under the query rows'
+// traffic: all kv heads first measured 79 us for 6 x 1000 tokens into Q8 pages).
 template <int V, typename T, bool Q8>
 __global__ void __launch_bounds__(kRopeThreads) b200q_rope_append_kernel(const AppendArgs a) {
-    __shared__ float2 cs[kMaxRot / 2];
-    __shared__ double2 cs64[Q8 ? kMaxRot / 2 : 1];
+    __shared__ float2 cs[kMaxRows * kMaxRot / 2];
+    __shared__ double2 cs64[Q8 ? kMaxRows * 64 : 1];  // head <= 128
+    __shared__ int2 place[kMaxRows];  // position and sequence of each row
+    __shared__ uint32_t pool_of[kMaxRows];  // pool row of kv head 0 at the position; kNoRow without a page
     griddep_launch_dependents();
     griddep_wait();
-    const int row = blockIdx.x;
-    const int b = seq_of_row(a.r, row);
-    if (b < 0) return;
-    const int2 rr = seq_rows(a.r, b);
-    const int pos = a.r.kv_len[b] - (rr.y - row);
-    const int np = a.s.rot / 2;
-    const bool keys = blockIdx.y == 0;
-    for (int i = threadIdx.x; i < np; i += kRopeThreads) {
-        cs[i] = cos_sin(pos, a.turns[i], static_cast<float>(a.mag));
-        if constexpr (Q8) {
-            if (keys) cs64[i] = cos_sin64(pos, a.turns[i], a.mag);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int np = a.s.rot / 2, hd = a.s.hd;
+    const int block = blockIdx.x / a.ctas, part = blockIdx.x - block * a.ctas;
+    const int r0 = block * a.rows_per_cta, nr = min(a.rows_per_cta, a.r.n_tokens - r0);
+    const bool keys = part < a.kv_ctas;
+    for (int i = warp; i < nr; i += kRopeThreads / 32) {
+        const int2 at = locate(a.r, r0 + i, lane);
+        if (lane == 0) {
+            place[i] = at;
+            uint32_t row = kNoRow;
+            if (keys && at.y >= 0) {
+                const int pg = at.x >= 0 ? at.x / a.kv.page : -1;
+                const int slot = page_slot(a.kv, at.y, pg);
+                if (slot >= 0) row = static_cast<uint32_t>(pool_row(a.kv, slot, 0, at.x - pg * a.kv.page));
+                else if (part == 0) flag_bad_page(a.kv);
+            }
+            pool_of[i] = row;
         }
     }
     __syncthreads();
-    if (a.q_out) {
-        const int h0 = blockIdx.y * a.heads_per_cta;
-        const int n = min(a.heads_per_cta, a.heads - h0) * a.s.units;
-        const T* x = static_cast<const T*>(a.q) + row * a.q_stride + h0 * a.s.hd;
-        T* y = static_cast<T*>(a.q_out) + row * a.q_out_stride + h0 * a.s.hd;
-#pragma unroll 4
-        for (int i = threadIdx.x; i < n; i += kRopeThreads) {
-            const int h = i / a.s.units, u = i - h * a.s.units;
-            rope_unit<V>(a.s, cs, x + h * a.s.hd, y + h * a.s.hd, u);
+    const bool wide = Q8 && keys;
+    for (int i = threadIdx.x; i < nr * np; i += kRopeThreads) {
+        const int r = i / np, p = i - r * np;
+        if (wide) {
+            if constexpr (Q8) cs64[r * 64 + p] = cos_sin64(place[r].x, a.turns[p], a.mag);
+        } else {
+            cs[i] = cos_sin(place[r].x, a.turns[p], static_cast<float>(a.mag));
         }
     }
-    if (!keys) return;
-    const int pg = pos >= 0 ? pos / a.kv.page : -1;
-    const int slot = page_slot(a.kv, b, pg);
-    if (slot < 0) {
-        if (threadIdx.x == 0) flag_bad_page(a.kv);
+    __syncthreads();
+    if (!keys) {
+        const int h0 = (part - a.kv_ctas) * a.heads_per_cta;
+        if (!a.walk) {
+            const int per_row = min(a.heads_per_cta, a.heads - h0) * a.s.units, total = nr * per_row;
+            const T* x = static_cast<const T*>(a.q) + r0 * a.q_stride + h0 * hd;
+            T* y = static_cast<T*>(a.q_out) + r0 * a.q_out_stride + h0 * hd;
+            for (int i0 = threadIdx.x; i0 < total; i0 += kRopeThreads * kAppendInFlight) {
+                RopeUnit<T, V> u[kAppendInFlight];
+                int at[kAppendInFlight], row[kAppendInFlight];
+#pragma unroll
+                for (int k = 0; k < kAppendInFlight; ++k) {
+                    int i = i0 + k * kRopeThreads;
+                    row[k] = -1;
+                    if (i >= total) continue;
+                    int r = 0;
+                    while (i >= per_row) i -= per_row, ++r;
+                    if (place[r].y < 0) continue;
+                    const int h = div_by(i, a.s.unit_mul, a.s.unit_shift);
+                    row[k] = r;
+                    at[k] = h * hd;
+                    u[k].load(a.s, x + r * a.q_stride + at[k], i - h * a.s.units);
+                }
+#pragma unroll
+                for (int k = 0; k < kAppendInFlight; ++k)
+                    if (row[k] >= 0) u[k].store(a.s, cs + row[k] * np, y + row[k] * a.q_out_stride + at[k]);
+            }
+            return;
+        }
+        for (int r = 0; r < nr; ++r)
+            if (place[r].y >= 0)
+                rotate_heads<V, kAppendInFlight>(
+                    a.s, cs + r * np, static_cast<const T*>(a.q) + (r0 + r) * a.q_stride + h0 * hd,
+                    static_cast<T*>(a.q_out) + (r0 + r) * a.q_out_stride + h0 * hd, static_cast<long long>(hd),
+                    min(a.heads_per_cta, a.heads - h0));
         return;
     }
-    const int off = pos - pg * a.kv.page;
-    const T* kin = static_cast<const T*>(a.k) + row * a.kv_stride;
-    const T* vin = static_cast<const T*>(a.v) + row * a.kv_stride;
-    const int hd = a.s.hd;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    // One warp per kv head's key or value row, lane l the elements l, l + 32, ...
-    for (int i = warp; i < 2 * a.kv.n_kv; i += kRopeThreads / 32) {
-        const bool is_v = i >= a.kv.n_kv;
-        const int h = is_v ? i - a.kv.n_kv : i;
-        const T* x = (is_v ? vin : kin) + h * hd;
-        const long long dst = pool_row(a.kv, slot, h, off);
-        constexpr int kMaxPer = 4;  // hd <= 128
-        float val[kMaxPer];
-        float amax = 0.0f;
+    const int kh0 = part * a.kv_per_cta;
+    const int nh = min(a.kv_per_cta, a.kv.n_kv - kh0);
+    if constexpr (!Q8) {
+        // Keys, then values (every unit a copy), of the rows' heads: too few per row
+        // to walk them row by row.
+        const int keys_of_row = nh * a.s.units, per_row = keys_of_row + nh * a.plain.units, total = nr * per_row;
+        for (int i0 = threadIdx.x; i0 < total; i0 += kRopeThreads * kAppendInFlight) {
+            RopeUnit<T, V> u[kAppendInFlight];
+            __half* dst[kAppendInFlight];
+            int row[kAppendInFlight];
 #pragma unroll
-        for (int t = 0; t < kMaxPer; ++t) {
-            const int e = lane + 32 * t;
-            val[t] = 0.0f;
-            if (e >= hd) continue;
-            val[t] = load1(x + e);
-            if (!is_v && e < a.s.rot) {
-                const int p = a.s.half ? (e < np ? e : e - np) : e >> 1;
-                const bool second = a.s.half ? e >= np : (e & 1);
-                const int mate = a.s.half ? (second ? e - np : e + np) : e ^ 1;
-                const float other = load1(x + mate);
-                if constexpr (Q8) {
-                    const double2 t2 = cs64[p];
-                    const double w = second ? other * t2.y + val[t] * t2.x : val[t] * t2.x - other * t2.y;
-                    val[t] = static_cast<float>(w);
-                } else {
-                    const float2 t2 = cs[p];
-                    val[t] = second ? other * t2.y + val[t] * t2.x : val[t] * t2.x - other * t2.y;
+            for (int k = 0; k < kAppendInFlight; ++k) {
+                int i = i0 + k * kRopeThreads;
+                dst[k] = nullptr;
+                if (i >= total) continue;
+                int r = 0;
+                while (i >= per_row) i -= per_row, ++r;
+                if (pool_of[r] == kNoRow) continue;
+                const bool is_v = i >= keys_of_row;
+                if (is_v) i -= keys_of_row;
+                const RopeShape& s = is_v ? a.plain : a.s;
+                const int h = div_by(i, s.unit_mul, s.unit_shift);
+                dst[k] = static_cast<__half*>(is_v ? a.kv.v : a.kv.k) +
+                         (pool_of[r] + static_cast<long long>(kh0 + h) * a.kv.page) * hd;
+                row[k] = r;
+                u[k].load(s, static_cast<const T*>(is_v ? a.v : a.k) + (r0 + r) * a.kv_stride + (kh0 + h) * hd,
+                          i - h * s.units);
+            }
+#pragma unroll
+            for (int k = 0; k < kAppendInFlight; ++k)
+                if (dst[k]) u[k].store(a.s, cs + row[k] * np, dst[k]);
+        }
+    } else {
+        // A row of a kv head's keys or values is E elements a lane, over hd / E
+        // lanes of a warp (so a warp takes two rows of 128, four of 64, at once);
+        // for the half layout a lane also reads its elements' mates.
+        constexpr int E = 8;
+        const int lanes = hd / E, sub = lane / lanes, e0 = lane % lanes * E;
+        const int tasks = nr * nh * 2, step = 32 / lanes * (kRopeThreads / 32);
+        for (int i0 = 0; i0 < tasks; i0 += step) {
+            int i = i0 + warp * (32 / lanes) + sub;
+            const bool mine = i < tasks;
+            i = mine ? i : 0;
+            int r = 0;
+            while (i >= 2 * nh) i -= 2 * nh, ++r;
+            const bool is_v = i >= nh;
+            const int h = kh0 + (is_v ? i - nh : i);
+            const T* src = static_cast<const T*>(is_v ? a.v : a.k) + (r0 + r) * a.kv_stride + h * hd;
+            float x[E], mate[E];
+            if (a.kv_wide) {
+                Vec<T, E> v, w;
+                v.load(src + e0);
+                const bool other = !is_v && a.s.half && e0 < a.s.rot;
+                if (other) w.load(src + (e0 < np ? e0 + np : e0 - np));
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    x[e] = v.get(e);
+                    mate[e] = other ? w.get(e) : v.get(e ^ 1);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const int el = e0 + e;
+                    x[e] = load1(src + el);
+                    mate[e] = 0.0f;
+                    if (!is_v && el < a.s.rot)
+                        mate[e] = load1(src + (a.s.half ? (el < np ? el + np : el - np) : el ^ 1));
                 }
             }
-            amax = fmaxf(amax, fabsf(val[t]));
-        }
-        if constexpr (Q8) {
+            float amax = 0.0f;
 #pragma unroll
-            for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+            for (int e = 0; e < E; ++e) {
+                const int el = e0 + e;
+                if (!is_v && el < a.s.rot) {
+                    const bool second = a.s.half ? el >= np : (el & 1);
+                    const double2 t = cs64[r * 64 + (a.s.half ? (second ? el - np : el) : el >> 1)];
+                    const double w = static_cast<double>(mate[e]) * t.y;
+                    x[e] = static_cast<float>(fma(static_cast<double>(x[e]), t.x, second ? w : -w));
+                }
+                amax = fmaxf(amax, fabsf(x[e]));
+            }
+            for (int o = lanes / 2; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
             const float scale = q8_scale(amax), inv = __fdiv_rn(1.0f, scale);
-            int8_t* out = static_cast<int8_t*>(is_v ? a.kv.v : a.kv.k) + dst * hd;
+            if (!mine || pool_of[r] == kNoRow) continue;
+            const long long dst = pool_of[r] + static_cast<long long>(h) * a.kv.page;
+            uint32_t lo = 0, up = 0;
 #pragma unroll
-            for (int t = 0; t < kMaxPer; ++t)
-                if (lane + 32 * t < hd) out[lane + 32 * t] = q8_code(val[t], inv);
-            if (lane == 0) (is_v ? a.kv.vs : a.kv.ks)[dst] = scale;
-        } else {
-            __half* out = static_cast<__half*>(is_v ? a.kv.v : a.kv.k) + dst * hd;
-#pragma unroll
-            for (int t = 0; t < kMaxPer; ++t)
-                if (lane + 32 * t < hd) out[lane + 32 * t] = __float2half_rn(val[t]);
+            for (int e = 0; e < 4; ++e) {
+                lo |= q8_code(x[e], inv) << (8 * e);
+                up |= q8_code(x[4 + e], inv) << (8 * e);
+            }
+            *reinterpret_cast<uint2*>(static_cast<int8_t*>(is_v ? a.kv.v : a.kv.k) + dst * hd + e0) = make_uint2(lo, up);
+            if (e0 == 0) (is_v ? a.kv.vs : a.kv.ks)[dst] = scale;
         }
     }
 }
@@ -307,16 +545,29 @@ cudaLaunchConfig_t ragged_cfg(dim3 grid, dim3 block, cudaStream_t st, cudaLaunch
 
 bool aligned_to(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
-// The units of one head, four elements wide when every vector of them stays
-// aligned (rows, heads and both halves of the pairs), else one pair.
-int rope_units(int hd, int rot, int half, bool wide, RopeShape& s) {
-    const int v = wide && hd % 4 == 0 && rot % (half ? 8 : 4) == 0 ? 4 : 1;
+// The units of one head: V elements wide (16 bytes, or 8 for fp16) when every
+// vector of them stays aligned -- rows, heads and both halves of the pairs --,
+// else one pair or element.
+int rope_units(int hd, int rot, int half, int v, RopeShape& s) {
+    while (v > 1 && (hd % v || rot % (half ? 2 * v : v))) v = v == 8 ? 4 : 1;
     s.hd = hd;
     s.rot = rot;
     s.half = half;
     s.pair_units = v == 1 ? rot / 2 : (half ? rot / 2 / v : rot / v);
     s.units = s.pair_units + (hd - rot) / v;
+    divisor(s.units, s.unit_mul, s.unit_shift);
     return v;
+}
+
+// The widest vector that pointers and strides (in elements) allow.
+int widest(size_t es, std::initializer_list<const void*> ptrs, std::initializer_list<long long> strides) {
+    for (int v = es == 2 ? 8 : 4; v > 1; v = v == 8 ? 4 : 1) {
+        bool ok = true;
+        for (const void* p : ptrs) ok = ok && aligned_to(p, v * es);
+        for (long long st : strides) ok = ok && st % v == 0;
+        if (ok) return v;
+    }
+    return 1;
 }
 
 size_t elem_size(int dtype) { return dtype == B200Q_F32 ? 4 : 2; }
@@ -390,19 +641,26 @@ int launch_rope_rows(const void* x, void* out, int dtype, int rows, int heads, i
     a.rows = rows;
     a.heads = heads;
     a.mag = static_cast<float>(mag);
-    const bool wide = aligned_to(x, 4 * es) && aligned_to(out, 4 * es) && x_stride % 4 == 0 && out_stride % 4 == 0;
-    const int v = rope_units(hd, rot, layout == B200Q_ROPE_HALF, wide, a.s);
-    a.rows_per_cta = 1;
-    a.heads_per_cta = heads;
+    const int v = rope_units(hd, rot, layout == B200Q_ROPE_HALF, widest(es, {x, out}, {x_stride, out_stride}), a.s);
+    // A CTA takes a few units a thread when there are many, one when the
+    // units would not give every SM a few CTAs.
+    const long long units = static_cast<long long>(rows) * heads * a.s.units;
+    const int per_cta = units > 2048ll * kRopeThreads ? kRowsInFlight * kRopeThreads : kRopeThreads;
+    a.heads_per_cta = std::max(1, std::min(heads, per_cta / a.s.units));
+    a.rows_per_cta = a.heads_per_cta < heads ? 1 : std::max(1, std::min(kMaxRows, per_cta / (heads * a.s.units)));
+    const int head_ctas = (heads + a.heads_per_cta - 1) / a.heads_per_cta;
+    if (head_ctas > 65535) return B200Q_ESHAPE;
     cudaLaunchAttribute attr[1];
-    cudaLaunchConfig_t cfg = ragged_cfg(dim3(rows, 1), dim3(kRopeThreads), st, attr);
+    cudaLaunchConfig_t cfg = ragged_cfg(dim3((rows + a.rows_per_cta - 1) / a.rows_per_cta, head_ctas),
+                                        dim3(kRopeThreads), st, attr);
     cudaError_t e;
     if (dtype == B200Q_F32)
         e = v == 4 ? cudaLaunchKernelEx(&cfg, b200q_rope_rows_kernel<4, float>, a)
                    : cudaLaunchKernelEx(&cfg, b200q_rope_rows_kernel<1, float>, a);
     else
-        e = v == 4 ? cudaLaunchKernelEx(&cfg, b200q_rope_rows_kernel<4, __half>, a)
-                   : cudaLaunchKernelEx(&cfg, b200q_rope_rows_kernel<1, __half>, a);
+        e = v == 8   ? cudaLaunchKernelEx(&cfg, b200q_rope_rows_kernel<8, __half>, a)
+            : v == 4 ? cudaLaunchKernelEx(&cfg, b200q_rope_rows_kernel<4, __half>, a)
+                     : cudaLaunchKernelEx(&cfg, b200q_rope_rows_kernel<1, __half>, a);
     return e == cudaSuccess ? B200Q_OK : B200Q_ECUDA;
 }
 
@@ -471,13 +729,32 @@ int launch_rope_append(const void* q, const void* k, const void* v, int dtype, i
     a.q_out_stride = q_out_stride;
     a.heads = heads;
     a.mag = mag;
-    const bool wide = !q_out || (aligned_to(q, 4 * es) && aligned_to(q_out, 4 * es) && q_stride % 4 == 0 &&
-                                 q_out_stride % 4 == 0);
-    const int vec = rope_units(hd, rot, layout == B200Q_ROPE_HALF, wide, a.s);
-    a.heads_per_cta = heads;
-    cudaLaunchAttribute attr[1];
-    cudaLaunchConfig_t cfg = ragged_cfg(dim3(n_tokens, 1), dim3(kRopeThreads), st, attr);
     const bool q8 = pkv.kv_mode == B200Q_KV_Q8;
+    int width = q_out ? widest(es, {q, q_out}, {q_stride, q_out_stride}) : 8;
+    // (Q8 rows are read by the warp that quantizes them, in its own widths.)
+    if (!q8) width = std::min(width, widest(es, {k, v}, {kv_stride}));
+    const int vec = rope_units(hd, rot, layout == B200Q_ROPE_HALF, std::min(width, es == 2 ? 8 : 4), a.s);
+    rope_units(hd, 0, 0, vec, a.plain);
+    const long long units = static_cast<long long>(n_tokens) * (q_out ? heads : pkv.n_kv) * a.s.units;
+    const bool many = units > 2048ll * kRopeThreads;
+    // Rows of many heads are walked (fewer instructions a unit), rows of few taken
+    // together (7 x 1200 rows of 144 units: 22 us against 33).
+    a.walk = many && heads * a.s.units >= kHeadsPerThread / 2 * kRopeThreads;
+    const int per_cta = (a.walk ? kHeadsPerThread : many ? kAppendInFlight : 1) * kRopeThreads;
+    a.heads_per_cta = std::max(1, std::min(heads, per_cta / a.s.units));
+    const int q_ctas = q_out ? (heads + a.heads_per_cta - 1) / a.heads_per_cta : 0;
+    a.rows_per_cta = std::min<long long>(kMaxRows, std::max<long long>(1, n_tokens / 2048));
+    a.kv_per_cta = std::max(1, std::min(pkv.n_kv, (many ? 2 : 1) * kRopeThreads / (2 * a.s.units)));
+    a.kv_ctas = (pkv.n_kv + a.kv_per_cta - 1) / a.kv_per_cta;
+    a.ctas = q_ctas + a.kv_ctas;
+    const long long blocks = (n_tokens + a.rows_per_cta - 1ll) / a.rows_per_cta;
+    if (blocks * a.ctas > 0x7fffffffll) return B200Q_ESHAPE;
+    // A lane's eight elements stay aligned, are all rotated or none, and so are
+    // their mates half the pairs away.
+    a.kv_wide = aligned_to(k, 16) && aligned_to(v, 16) && kv_stride % 8 == 0 &&
+                rot % (layout == B200Q_ROPE_HALF ? 16 : 8) == 0;
+    cudaLaunchAttribute attr[1];
+    cudaLaunchConfig_t cfg = ragged_cfg(dim3(static_cast<unsigned>(blocks * a.ctas)), dim3(kRopeThreads), st, attr);
     cudaError_t e;
 #define B200Q_APPEND(V, T)                                                       \
     e = q8 ? cudaLaunchKernelEx(&cfg, b200q_rope_append_kernel<V, T, true>, a)   \
@@ -486,7 +763,8 @@ int launch_rope_append(const void* q, const void* k, const void* v, int dtype, i
         if (vec == 4) B200Q_APPEND(4, float);
         else B200Q_APPEND(1, float);
     } else {
-        if (vec == 4) B200Q_APPEND(4, __half);
+        if (vec == 8) B200Q_APPEND(8, __half);
+        else if (vec == 4) B200Q_APPEND(4, __half);
         else B200Q_APPEND(1, __half);
     }
 #undef B200Q_APPEND

@@ -12,6 +12,8 @@
 
 namespace b200q {
 
+constexpr uint32_t kNoRow = 0xFFFFFFFFu;  // a pool row that is none
+
 struct RaggedView {
     const int* cu_q;    // [batch + 1] first row of each sequence
     const int* kv_len;  // [batch] positions of the sequence, this batch's tokens included
@@ -32,24 +34,48 @@ struct PagedView {
     volatile int* status;
 };
 
+// x / d for 0 <= x < 2^31: umulhi(2 x, mul) >> shift, shift = ceil(log2 d), mul
+// = ceil(2^(31 + shift) / d) (its excess e < d adds less than x e / (d
+// 2^(31 + shift)) < 1 / d to the quotient).
+__device__ __forceinline__ int div_by(int x, uint32_t mul, int shift) {
+    return static_cast<int>(__umulhi(2u * static_cast<uint32_t>(x), mul) >> shift);
+}
+
+inline void divisor(int d, uint32_t& mul, int& shift) {
+    shift = 0;
+    while ((1ll << shift) < d) ++shift;
+    mul = static_cast<uint32_t>(((1ull << (31 + shift)) + d - 1) / d);
+}
+
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<uint64_t&>(d))
+        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<uint64_t&>(d))
+        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<uint64_t&>(d))
+        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+    return d;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
 // Rows of sequence b, clamped to the rows that exist (cu_q is the caller's).
 __device__ __forceinline__ int2 seq_rows(const RaggedView& r, int b) {
     const int lo = min(max(r.cu_q[b], 0), r.n_tokens);
     const int hi = min(max(r.cu_q[b + 1], lo), r.n_tokens);
     return make_int2(lo, hi);
-}
-
-// The sequence that holds row `row`: the last b with cu_q[b] <= row; -1 when
-// the row belongs to none.
-__device__ __forceinline__ int seq_of_row(const RaggedView& r, int row) {
-    int lo = 0, hi = r.batch;  // cu_q[lo] <= row < cu_q[hi], if any
-    if (row < r.cu_q[0] || row >= r.cu_q[r.batch]) return -1;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (r.cu_q[mid] <= row) lo = mid;
-        else hi = mid;
-    }
-    return lo;
 }
 
 // Pool slot of page `pg` of sequence b: -1 for a page not assigned, -2 for

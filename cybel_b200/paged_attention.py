@@ -21,12 +21,13 @@ from __future__ import annotations
 import ctypes
 import math
 
+import numpy as np
+import torch
+
 from . import _native
 
 
 def _cuda_index(device):
-    import torch
-
     dev = torch.device("cuda", device) if isinstance(device, int) else torch.device(device)
     if dev.type == "cuda" and dev.index is None:
         dev = torch.device("cuda", torch.cuda.current_device())
@@ -49,9 +50,6 @@ class RopeTable:
     def __init__(self, rot_dim: int, theta: float = 10000.0, layout: str = "interleaved", scaling: str = "none",
                  factor: float = 1.0, original_context: int = 0, low: float | None = None, high: float | None = None,
                  device: int | str = 0):
-        import numpy as np
-        import torch
-
         if layout not in _native.ROPE_LAYOUTS:
             raise ValueError(f"unknown rotary layout {layout!r}")
         if scaling not in _native.ROPE_SCALINGS:
@@ -70,28 +68,24 @@ class RopeTable:
         self.dev = _cuda_index(device)
         self.turns = torch.from_numpy(turns.view(np.int64)).to(self.dev)
         self._ptr, self._layout = self.turns.data_ptr(), _native.ROPE_LAYOUTS[layout]
+        self._index = device_index(self.dev)
 
     def rotate(self, x, positions, out=None):
         """x [rows][heads][head_dim] (fp32 or fp16, heads packed) rotated to
         ``positions`` (int32 [rows], >= 0) into ``out`` (a new tensor when
         None; may be x). Current stream; b200q_rope_rows."""
-        import torch
-
         if out is None:
             out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        dt, xs, os_ = _dtype(x), _row_stride(x, "x"), _row_stride(out, "out")
-        if out.shape != x.shape or out.dtype != x.dtype:
+        dt, shape, xs = _rows(x, "x", self._index)
+        odt, oshape, os_ = _rows(out, "out", self._index)
+        if oshape != shape or odt != dt:
             raise ValueError("out must have x's shape and type")
-        n, heads, hd = x.shape
+        n, heads, hd = shape
         if hd < self.rot_dim:
             raise ValueError("heads smaller than the table's rot_dim")
-        if positions.dtype != torch.int32 or positions.shape != (n,) or not positions.is_contiguous():
-            raise ValueError("positions must be contiguous int32 [rows]")
-        _same_device(self.dev, x, out, positions)
-        with _on(self.dev):
-            _native.check(_native.lib().b200q_rope_rows(
-                x.data_ptr(), out.data_ptr(), dt, n, heads, hd, xs, os_, positions.data_ptr(), self._ptr, self.rot_dim,
-                self._layout, self.mag, _stream(self.dev)), "rotary rows")
+        _vector(positions, "positions", torch.int32, n, self._index)
+        _call(self._index, _native.lib().b200q_rope_rows, "rotary rows", x.data_ptr(), out.data_ptr(), dt, n, heads,
+              hd, xs, os_, positions.data_ptr(), self._ptr, self.rot_dim, self._layout, self.mag)
         return out
 
 
@@ -107,9 +101,8 @@ class RaggedBatch:
     a batch that grows is made with."""
 
     def __init__(self, q_lens, kv_lens, device: int | str = 0, max_q: int | None = None, max_kv: int | None = None):
-        import torch
-
         self.dev = _cuda_index(device)
+        self._index = device_index(self.dev)
         q, kv = self._checked(q_lens, kv_lens)
         self.batch, self.n_tokens = len(q), sum(q)
         self.max_q = max(q) if max_q is None else int(max_q)
@@ -130,8 +123,6 @@ class RaggedBatch:
         return q, kv
 
     def update(self, q_lens, kv_lens) -> None:
-        import torch
-
         q, kv = self._checked(q_lens, kv_lens)
         if len(q) != self.batch or sum(q) > self.n_tokens or max(q) > self.max_q or max(kv) > self.max_kv:
             raise ValueError("lengths past those the batch was made for")
@@ -143,15 +134,12 @@ class RaggedBatch:
         self.kv_len.copy_(torch.tensor(kv, dtype=torch.int32))
 
 
-# ---- argument checks ----------------------------------------------------------
-def _dtype(t) -> int:
-    import torch
-
-    if t.dtype == torch.float32:
-        return _native.F32
-    if t.dtype == torch.float16:
-        return _native.F16
-    raise ValueError("activation rows must be fp32 or fp16")
+# ---- argument checks and the call ---------------------------------------------
+# These run before every launch of a decode step, whose kernels take 2-9 us:
+# they ask torch for each property once and make no objects they can do without.
+def device_index(dev) -> int:
+    """Ordinal of a CUDA device, -1 for the host (as Tensor.get_device)."""
+    return dev.index if dev.type == "cuda" else -1
 
 
 def _row_stride(t, name: str) -> int:
@@ -161,119 +149,118 @@ def _row_stride(t, name: str) -> int:
         raise ValueError(f"{name} must be [rows][heads][head_dim]")
     n, h, d = t.shape
     s0, s1, s2 = t.stride()
-    if (s2 != 1 and d > 1) or (s1 != d and h > 1) or (n > 1 and s0 < h * d):
+    if n <= 1:
+        s0 = h * d
+    if (s2 != 1 and d > 1) or (s1 != d and h > 1) or s0 < h * d:
         raise ValueError(f"{name}: the heads of a row must be packed and its rows apart")
-    return s0 if n > 1 else h * d
+    return s0
 
 
-def _same_device(dev, *tensors) -> None:
-    for t in tensors:
-        if t.device != dev:
-            raise ValueError(f"tensors on {t.device} and {dev}")
+def _rows(t, name: str, index: int):
+    """(element type, shape, row stride) of activation rows on device `index`."""
+    dtype = t.dtype
+    if dtype is torch.float32:
+        dt = _native.F32
+    elif dtype is torch.float16:
+        dt = _native.F16
+    else:
+        raise ValueError(f"{name}: activation rows must be fp32 or fp16")
+    stride = _row_stride(t, name)
+    if t.get_device() != index:
+        raise ValueError(f"{name} is on another device")
+    return dt, t.shape, stride
 
 
-class _Here:
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *exc):
-        return False
-
-
-_HERE = _Here()
+def _vector(t, name: str, dtype, n: int, index: int) -> None:
+    if t.dtype is not dtype or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous {dtype} [{n}]")
+    if t.get_device() != index:
+        raise ValueError(f"{name} is on another device")
 
 
-def _on(dev):
-    """The tensors' device made current for the call (where it is not)."""
-    import torch
-
-    if dev.type != "cuda":
+def _call(index: int, fn, what: str, *args) -> None:
+    """fn(*args, stream) on the current stream of device `index`, which is
+    made current for the call where it is not."""
+    if index < 0:
         raise RuntimeError("the ragged operators run on a CUDA device")
-    return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+    # (the handle itself: torch.cuda.current_stream makes a Stream object, 2 us)
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, stream)
+    if rc:
+        raise _native.NativeError(rc, what)
 
 
-def _stream(dev) -> int:
-    import torch
-
-    return torch.cuda.current_stream(dev).cuda_stream
-
-
-def _check_batch(cache, batch, rows: int) -> None:
+def _check_batch(cache, batch, rows: int, index: int) -> None:
     if batch.batch != cache.batch:
         raise ValueError("the ragged batch has another number of sequences than the cache")
     if rows != batch.n_tokens:
         raise ValueError("rows and the batch's tokens differ")
     if batch.max_kv > cache.pages_per_seq * cache.page_size:
         raise ValueError("lengths past the cache")
-    _same_device(cache.dev, batch.kv_len)
+    if batch._index != index:
+        raise ValueError("the batch is on another device")
 
 
 def append(cache, layer, k, v, batch, rope=None, q=None, q_out=None):
     """PagedKVCache.append."""
-    import torch
-
-    dt = _dtype(k)
-    ks, vs = _row_stride(k, "k"), _row_stride(v, "v")
-    shape = (batch.n_tokens, cache.kv_heads, cache.head_dim)
-    if k.shape != shape or v.shape != shape or v.dtype != k.dtype or (ks != vs and k.shape[0] > 1):
+    index = device_index(cache.dev)
+    dt, shape, ks = _rows(k, "k", index)
+    vdt, vshape, vs = _rows(v, "v", index)
+    n, kv_heads, hd = shape
+    if (kv_heads != cache.kv_heads or hd != cache.head_dim or vshape != shape or vdt != dt or (ks != vs and n > 1)):
         raise ValueError("k and v must be [n_tokens][kv_heads][head_dim] of one type, rows equally far apart")
-    _check_batch(cache, batch, k.shape[0])
-    _same_device(cache.dev, k, v)
+    _check_batch(cache, batch, n, index)
     heads = qs = qos = 0
     if q is not None:
         if q_out is None:
             q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        qs, qos = _row_stride(q, "q"), _row_stride(q_out, "q_out")
-        if q.shape[0] != shape[0] or q.shape[2] != shape[2] or q.dtype != k.dtype:
+        qdt, qshape, qs = _rows(q, "q", index)
+        odt, oshape, qos = _rows(q_out, "q_out", index)
+        if qshape[0] != n or qshape[2] != hd or qdt != dt:
             raise ValueError("q must be [n_tokens][heads][head_dim] of k's type")
-        if q_out.shape != q.shape or q_out.dtype != q.dtype:
+        if oshape != qshape or odt != dt:
             raise ValueError("q_out must have q's shape and type")
-        _same_device(cache.dev, q, q_out)
-        heads = q.shape[1]
+        heads = qshape[1]
     elif q_out is not None:
         raise ValueError("q_out without q")
     turns, rot, layout, mag = None, 0, 0, 1.0
     if rope is not None:
-        if rope.rot_dim > cache.head_dim:
+        if rope.rot_dim > hd:
             raise ValueError("heads smaller than the table's rot_dim")
-        _same_device(cache.dev, rope.turns)
+        if rope._index != index:
+            raise ValueError("the rotary table is on another device")
         turns, rot, layout, mag = rope._ptr, rope.rot_dim, rope._layout, rope.mag
-    with _on(cache.dev):
-        _native.check(_native.lib().b200q_rope_append_paged(
-            q.data_ptr() if heads else None, k.data_ptr(), v.data_ptr(), dt, shape[0], batch.batch,
-            batch.cu_q.data_ptr(), batch.kv_len.data_ptr(), heads, cache.kv_heads, cache.head_dim, qs, ks,
-            q_out.data_ptr() if heads else None, qos, turns, rot, layout, mag, *cache._pools(layer),
-            _stream(cache.dev)), "paged append")
+    _call(index, _native.lib().b200q_rope_append_paged, "paged append", q.data_ptr() if heads else None, k.data_ptr(),
+          v.data_ptr(), dt, n, batch.batch, batch.cu_q.data_ptr(), batch.kv_len.data_ptr(), heads, kv_heads, hd, qs,
+          ks, q_out.data_ptr() if heads else None, qos, turns, rot, layout, mag, *cache._pools(layer))
     return q_out
 
 
 def attend(cache, layer, q, batch, out=None, scale=None, softcap=0.0, slopes=None, window=0, prefix=None):
     """PagedKVCache.attend."""
-    import torch
-
+    index = device_index(cache.dev)
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    dt, qs, os_ = _dtype(q), _row_stride(q, "q"), _row_stride(out, "out")
-    n, heads, hd = q.shape
+    dt, shape, qs = _rows(q, "q", index)
+    odt, oshape, os_ = _rows(out, "out", index)
+    n, heads, hd = shape
     if hd != cache.head_dim or heads % cache.kv_heads:
         raise ValueError("q must be [n_tokens][heads][head_dim], heads a multiple of the cache's")
-    if out.shape != q.shape or out.dtype != q.dtype:
+    if oshape != shape or odt != dt:
         raise ValueError("out must have q's shape and type")
-    _check_batch(cache, batch, n)
-    _same_device(cache.dev, q, out)
+    _check_batch(cache, batch, n, index)
     if slopes is not None:
-        if slopes.dtype != torch.float32 or slopes.shape != (heads,) or not slopes.is_contiguous():
-            raise ValueError("slopes must be contiguous fp32 [heads]")
-        _same_device(cache.dev, slopes)
+        _vector(slopes, "slopes", torch.float32, heads, index)
+        slopes = slopes.data_ptr()
     if prefix is not None:
-        if prefix.dtype != torch.int32 or prefix.shape != (batch.batch,) or not prefix.is_contiguous():
-            raise ValueError("prefix must be contiguous int32 [sequences]")
-        _same_device(cache.dev, prefix)
-    with _on(cache.dev):
-        _native.check(_native.lib().b200q_attention_paged(
-            q.data_ptr(), dt, n, batch.batch, batch.cu_q.data_ptr(), batch.kv_len.data_ptr(), batch.max_q,
-            batch.max_kv, heads, cache.kv_heads, hd, qs, out.data_ptr(), os_,
-            1.0 / math.sqrt(hd) if scale is None else float(scale), float(softcap),
-            None if slopes is None else slopes.data_ptr(), int(window), None if prefix is None else prefix.data_ptr(),
-            *cache._pools(layer), _stream(cache.dev)), "paged attention")
+        _vector(prefix, "prefix", torch.int32, batch.batch, index)
+        prefix = prefix.data_ptr()
+    _call(index, _native.lib().b200q_attention_paged, "paged attention", q.data_ptr(), dt, n, batch.batch,
+          batch.cu_q.data_ptr(), batch.kv_len.data_ptr(), batch.max_q, batch.max_kv, heads, cache.kv_heads, hd, qs,
+          out.data_ptr(), os_, 1.0 / math.sqrt(hd) if scale is None else scale, softcap, slopes, window, prefix,
+          *cache._pools(layer))
     return out
