@@ -33,8 +33,7 @@ namespace b200q {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kTile = 16;        // positions per tile
-constexpr int kMaxCluster = 8;
+constexpr int kMaxCluster = 16;  // beyond 8 only where the device allows it
 constexpr float kRise = 4.0f;    // a row's reference maximum follows once exceeded by this (log2)
 constexpr float kLift = 10.0f;   // weights are 2^(score - maximum + kLift): at most 2^14 in fp16
 
@@ -43,14 +42,21 @@ struct Few {
     static constexpr int R = PREC ? 8 : 16;               // rows per block
     static constexpr int RB = Q8 ? D : 2 * D;             // bytes per stored row
     static constexpr int CH = RB / 16;                    // 16-byte chunks per row
+    // Positions per tile: more of them give a warp more independent products;
+    // rows of 256 bytes leave room for 16 only.
+    static constexpr int kTile = RB == 256 ? 16 : 32;
     static constexpr int kScales = Q8 ? 2 * kTile * 4 : 0;  // the tile's key and value scales
     static constexpr int kStage = 2 * kTile * RB + kScales;
-    static constexpr int NS = RB == 256 ? 3 : (RB == 128 ? 5 : 6);
+    static constexpr int NS = RB == 128 ? 2 : 3;
     static constexpr int kRing = NS * kStage;
     static constexpr int kPart = R * D * 4;               // a warp's output, in its ring after the loop
     static constexpr int kWarpBytes = kRing > kPart ? kRing : kPart;
     static constexpr int kTotal = kWarps * kWarpBytes + kWarps * R * 8 + R * 8;
 };
+
+// Resident CTAs per SM: rows of 256 bytes fill the shared memory with two.
+template <int D, bool Q8>
+constexpr int kCtasPerSm = (Q8 ? D : 2 * D) == 256 ? 2 : 3;
 
 __device__ __forceinline__ void ldsm4(uint32_t (&v)[4], uint32_t a) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -70,6 +76,11 @@ __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uin
         "%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float2 lds_f2(uint32_t a) {
+    float2 v;
+    asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a));
+    return v;
 }
 __device__ __forceinline__ uint32_t pack2(float x, float y) {
     const __half2 h = __floats2half2_rn(x, y);
@@ -105,10 +116,12 @@ __device__ __forceinline__ int v_chunk(int r, int c) {
 }
 
 template <int D, bool PREC, bool Q8>
-__global__ void __launch_bounds__(kWarps * 32, 2) b200q_attn_few_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(kWarps * 32, kCtasPerSm<D, Q8>) b200q_attn_few_kernel(const AttnArgs a) {
     using F = Few<D, PREC, Q8>;
     using T = typename std::conditional<PREC, float, __half>::type;
-    constexpr int R = F::R, KS = D / 16, NB = D / 8, NS = F::NS;
+    constexpr int R = F::R, KS = D / 16, NB = D / 8, NS = F::NS, kTile = F::kTile;
+    constexpr int NK = kTile / 8;  // blocks of 8 positions
+    constexpr uint32_t kAll = kTile == 32 ? 0xFFFFFFFFu : 0xFFFFu;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint32_t present[kWarps][8];  // per stage: which of its 16 positions have a row
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
@@ -207,10 +220,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2) b200q_attn_few_kernel(const At
     const int n_mine = p_hi < 0 || tiles.count <= first ? 0 : (tiles.count - first + stride - 1) / stride;
     const int hi_seen = max(p_hi, s.pre - 1), lo_seen = s.first(max(p_lo, 0));
 
-    // Position lane % 16 of my tile i: its pool row, if some row of the block sees it.
+    // Position lane % kTile of my tile i: its pool row, if some row of the block sees it.
     auto look = [&](int i) -> uint32_t {
         if (i >= n_mine) return kNoRow;
-        const int j = tiles.at(first + i * stride) + (lane & 15);
+        const int j = tiles.at(first + i * stride) + lane % kTile;
         return (j <= hi_seen && (j < s.pre || j >= lo_seen)) ? row_of(a, b, kvh, j) : kNoRow;
     };
     uint32_t ahead = look(0);  // row of the next tile to load
@@ -232,12 +245,13 @@ __global__ void __launch_bounds__(kWarps * 32, 2) b200q_attn_few_kernel(const At
                            static_cast<const uint8_t*>(a.kv.v) + off, ok);
             }
             if constexpr (Q8) {
+                static_assert(!Q8 || kTile == 32, "a lane per position");
                 const bool ok = rowi != kNoRow;
-                const float* src = lane < kTile ? a.kv.ks : a.kv.vs;
-                cp_async4(st + 2 * kTile * F::RB + lane * 4, src + (ok ? rowi : 0), ok);
+                cp_async4(st + 2 * kTile * F::RB + lane * 4, a.kv.ks + (ok ? rowi : 0), ok);
+                cp_async4(st + 2 * kTile * F::RB + (kTile + lane) * 4, a.kv.vs + (ok ? rowi : 0), ok);
             }
         }
-        const uint32_t bits = __ballot_sync(0xffffffffu, rowi != kNoRow) & 0xFFFFu;
+        const uint32_t bits = __ballot_sync(0xffffffffu, rowi != kNoRow) & kAll;
         if (lane == 0) present[warp][i % NS] = bits;
         cp_async_commit();
     };
@@ -252,42 +266,62 @@ __global__ void __launch_bounds__(kWarps * 32, 2) b200q_attn_few_kernel(const At
         const uint32_t kt = st, vt = st + kTile * F::RB;
         const uint32_t bits = present[warp][i % NS];
         const int j0 = tiles.at(first + i * stride);
-        // ---- scores: S[rows][16 positions]
-        float sc[2][4];
+        // ---- scores: S[rows][positions], with 16 positions in two halves of the
+        // head, so that four chains of products run side by side
+        constexpr int HV = NK == 2 ? 2 : 1;
+        float sc[NK][4];
+        {
+            float acc[HV][NK][4];
 #pragma unroll
-        for (int nb = 0; nb < 2; ++nb) {
-            sc[nb][0] = sc[nb][1] = sc[nb][2] = sc[nb][3] = 0.0f;
+            for (int hv = 0; hv < HV; ++hv)
+#pragma unroll
+                for (int nb = 0; nb < NK; ++nb) acc[hv][nb][0] = acc[hv][nb][1] = acc[hv][nb][2] = acc[hv][nb][3] = 0.0f;
             if constexpr (!Q8) {
 #pragma unroll
-                for (int ks = 0; ks < KS; ks += 2) {
-                    uint32_t k4[4];
-                    const int r = nb * 8 + (lane & 7);
-                    ldsm4(k4, kt + r * F::RB + k_chunk<D, Q8>(r, ks * 2 + (lane >> 3)) * 16);
-                    mma16(sc[nb], qa[ks], k4[0], k4[1]);
-                    mma16(sc[nb], qa[ks + 1], k4[2], k4[3]);
-                }
+                for (int ks = 0; ks < KS / HV; ks += 2)
+#pragma unroll
+                    for (int nb = 0; nb < NK; ++nb)
+#pragma unroll
+                        for (int hv = 0; hv < HV; ++hv) {
+                            uint32_t k4[4];
+                            const int r = nb * 8 + (lane & 7), kk = hv * (KS / 2) + ks;
+                            ldsm4(k4, kt + r * F::RB + k_chunk<D, Q8>(r, kk * 2 + (lane >> 3)) * 16);
+                            mma16(acc[hv][nb], qa[kk], k4[0], k4[1]);
+                            mma16(acc[hv][nb], qa[kk + 1], k4[2], k4[3]);
+                        }
             } else {
-                const int r = nb * 8 + g;
 #pragma unroll
                 for (int kq = 0; kq < D / 64; ++kq) {
-                    const uint4 w = lds128(kt + r * F::RB + k_chunk<D, Q8>(r, kq * 4 + c) * 16);
-                    const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+                    uint4 w[NK];
 #pragma unroll
-                    for (int t = 0; t < 4; ++t) {
-                        const uint32_t u = ww[t] ^ 0x80808080u;
-                        mma16(sc[nb], qa[kq * 4 + t], codes_fp16(u, 0x4140), codes_fp16(u, 0x4342));
+                    for (int nb = 0; nb < NK; ++nb) {
+                        const int r = nb * 8 + g;
+                        w[nb] = lds128(kt + r * F::RB + k_chunk<D, Q8>(r, kq * 4 + c) * 16);
                     }
+#pragma unroll
+                    for (int t = 0; t < 4; ++t)
+#pragma unroll
+                        for (int nb = 0; nb < NK; ++nb) {
+                            const uint32_t u =
+                                (t == 0 ? w[nb].x : t == 1 ? w[nb].y : t == 2 ? w[nb].z : w[nb].w) ^ 0x80808080u;
+                            mma16(acc[0][nb], qa[kq * 4 + t], codes_fp16(u, 0x4140), codes_fp16(u, 0x4342));
+                        }
                 }
             }
+#pragma unroll
+            for (int nb = 0; nb < NK; ++nb)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) sc[nb][v] = HV == 2 ? acc[0][nb][v] + acc[HV - 1][nb][v] : acc[0][nb][v];
         }
         // ---- exponents (log2); position of value v of block nb: j0 + 8 nb + 2 c + (v & 1)
-        float x[NR][4];
+        constexpr int NX = 2 * NK;
+        float x[NR][NX];
 #pragma unroll
-        for (int nb = 0; nb < 2; ++nb) {
+        for (int nb = 0; nb < NK; ++nb) {
             float ks0 = 1.0f, ks1 = 1.0f;
             if constexpr (Q8) {
-                ks0 = __uint_as_float(lds32(st + 2 * kTile * F::RB + (nb * 8 + 2 * c) * 4));
-                ks1 = __uint_as_float(lds32(st + 2 * kTile * F::RB + (nb * 8 + 2 * c + 1) * 4));
+                const float2 k2 = lds_f2(st + 2 * kTile * F::RB + (nb * 8 + 2 * c) * 4);
+                ks0 = k2.x, ks1 = k2.y;
             }
             if constexpr (PREC) {
                 x[0][2 * nb] = (sc[nb][0] + sc[nb][2]) * ks0;
@@ -297,15 +331,15 @@ __global__ void __launch_bounds__(kWarps * 32, 2) b200q_attn_few_kernel(const At
                 x[NR - 1][2 * nb] = sc[nb][2] * ks0, x[NR - 1][2 * nb + 1] = sc[nb][3] * ks1;
             }
         }
-        const bool whole = bits == 0xFFFFu && s.all(p_lo, p_hi, j0, j0 + kTile - 1);
+        const bool whole = bits == kAll && s.all(p_lo, p_hi, j0, j0 + kTile - 1);
 #pragma unroll
         for (int i2 = 0; i2 < NR; ++i2) {
 #pragma unroll
-            for (int v = 0; v < 4; ++v) x[i2][v] *= mult[i2];
+            for (int v = 0; v < NX; ++v) x[i2][v] *= mult[i2];
             if (shaped) {
                 if (a.cap > 0.0f) {
 #pragma unroll
-                    for (int v = 0; v < 4; v += 2) {
+                    for (int v = 0; v < NX; v += 2) {
                         const float2 z = mul2(make_float2(x[i2][v], x[i2][v + 1]), both(inv_cap));
                         const float2 near = tanh_near(z);
                         x[i2][v] = a.cap * (fabsf(z.x) > 1.0f ? tanh_far(z.x) : near.x);
@@ -313,14 +347,14 @@ __global__ void __launch_bounds__(kWarps * 32, 2) b200q_attn_few_kernel(const At
                     }
                 }
 #pragma unroll
-                for (int v = 0; v < 4; ++v) {
+                for (int v = 0; v < NX; ++v) {
                     const int j = j0 + 8 * (v >> 1) + 2 * c + (v & 1);
                     x[i2][v] = x[i2][v] * kLog2e - slope[i2] * fabsf(static_cast<float>(pos[i2] - j));
                 }
             }
             if (!whole) {
 #pragma unroll
-                for (int v = 0; v < 4; ++v) {
+                for (int v = 0; v < NX; ++v) {
                     const int jj = 8 * (v >> 1) + 2 * c + (v & 1);
                     if (!((bits >> jj) & 1u) || !s.sees(pos[i2], j0 + jj)) x[i2][v] = -INFINITY;
                 }
@@ -332,27 +366,28 @@ __global__ void __launch_bounds__(kWarps * 32, 2) b200q_attn_few_kernel(const At
 #pragma unroll
         for (int i2 = 0; i2 < NR; ++i2) {
             top[i2] = fmaxf(fmaxf(x[i2][0], x[i2][1]), fmaxf(x[i2][2], x[i2][3]));
+#pragma unroll
+            for (int v = 4; v < NX; ++v) top[i2] = fmaxf(top[i2], x[i2][v]);
             top[i2] = fmaxf(top[i2], __shfl_xor_sync(0xffffffffu, top[i2], 1));
             top[i2] = fmaxf(top[i2], __shfl_xor_sync(0xffffffffu, top[i2], 2));
             rise |= top[i2] > m[i2] + kRise;
         }
         float unit = 1.0f;  // Q8: change of o's unit
-        float vs[4];
+        float vs[NX];
         if constexpr (Q8) {
-            const float mine = __uint_as_float(lds32(st + 2 * kTile * F::RB + (kTile + (lane & 15)) * 4));
-            float mx = fabsf(mine) < INFINITY ? fabsf(mine) : 0.0f;
+            const float mine = fabsf(__uint_as_float(lds32(st + 2 * kTile * F::RB + (kTile + lane) * 4)));
+            const float mx = mine < INFINITY ? mine : 0.0f;
             if (__any_sync(0xffffffffu, mx >= E)) {
-#pragma unroll
-                for (int w = 8; w; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
-                const float e2 = pow2_above(mx);
+                const float e2 = pow2_above(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx))));
                 unit = E / e2;  // both powers of two (0 at the first tile, where o is 0)
                 E = e2;
                 inv_E = 1.0f / E;
             }
 #pragma unroll
-            for (int v = 0; v < 4; ++v)
-                vs[v] = __uint_as_float(lds32(st + 2 * kTile * F::RB + (kTile + 8 * (v >> 1) + 2 * c + (v & 1)) * 4)) *
-                        inv_E;
+            for (int nb = 0; nb < NK; ++nb) {
+                const float2 v2 = lds_f2(st + 2 * kTile * F::RB + (kTile + 8 * nb + 2 * c) * 4);
+                vs[2 * nb] = v2.x * inv_E, vs[2 * nb + 1] = v2.y * inv_E;
+            }
         }
         if (__any_sync(0xffffffffu, rise) || unit != 1.0f) {
 #pragma unroll
@@ -373,27 +408,30 @@ __global__ void __launch_bounds__(kWarps * 32, 2) b200q_attn_few_kernel(const At
                 }
             }
         }
-        // ---- weights
-        uint32_t pa[4];
+        // ---- weights, a fragment per 16 positions
+        uint32_t pa[kTile / 16][4];
 #pragma unroll
         for (int i2 = 0; i2 < NR; ++i2) {
             const float base = m[i2] == -INFINITY ? 0.0f : kLift - m[i2];
-            float p[4];
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                p[v] = ex2(x[i2][v] + base);
-                l[i2] += p[v];
-                if constexpr (Q8) p[v] = x[i2][v] == -INFINITY ? 0.0f : p[v] * vs[v];
-            }
-            if constexpr (PREC) {
-                pa[0] = pack2(p[0], p[1]);
-                pa[2] = pack2(p[2], p[3]);
-                const float2 h0 = unpack2(pa[0]), h1 = unpack2(pa[2]);
-                pa[1] = pack2(p[0] - h0.x, p[1] - h0.y);
-                pa[3] = pack2(p[2] - h1.x, p[3] - h1.y);
-            } else {
-                pa[i2] = pack2(p[0], p[1]);
-                pa[2 + i2] = pack2(p[2], p[3]);
+            for (int f = 0; f < kTile / 16; ++f) {
+                float p[4];
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                    p[v] = ex2(x[i2][4 * f + v] + base);
+                    l[i2] += p[v];
+                    if constexpr (Q8) p[v] = x[i2][4 * f + v] == -INFINITY ? 0.0f : p[v] * vs[4 * f + v];
+                }
+                if constexpr (PREC) {
+                    pa[f][0] = pack2(p[0], p[1]);
+                    pa[f][2] = pack2(p[2], p[3]);
+                    const float2 h0 = unpack2(pa[f][0]), h1 = unpack2(pa[f][2]);
+                    pa[f][1] = pack2(p[0] - h0.x, p[1] - h0.y);
+                    pa[f][3] = pack2(p[2] - h1.x, p[3] - h1.y);
+                } else {
+                    pa[f][i2] = pack2(p[0], p[1]);
+                    pa[f][2 + i2] = pack2(p[2], p[3]);
+                }
             }
         }
         if constexpr (!Q8) {
@@ -436,43 +474,46 @@ __global__ void __launch_bounds__(kWarps * 32, 2) b200q_attn_few_kernel(const At
             }
         }
         // ---- O += P V
-        if constexpr (!Q8) {
 #pragma unroll
-            for (int n = 0; n < NB; n += 2) {
-                uint32_t v4[4];
-                const int r = (lane & 7) + 8 * ((lane >> 3) & 1);
-                ldsm4t(v4, vt + r * F::RB + v_chunk<D, Q8>(r, n + (lane >> 4)) * 16);
-                mma16(o[n], pa, v4[0], v4[1]);
-                mma16(o[n + 1], pa, v4[2], v4[3]);
-            }
-        } else {
-            // Block n, column g: element g * NB + n, so that a lane's elements of a
-            // value are consecutive bytes.
-            constexpr int W = D / 32;  // 32-bit words per lane and value
-            uint32_t wv[4][W];
+        for (int f = 0; f < kTile / 16; ++f) {
+            const uint32_t vf = vt + f * 16 * F::RB;
+            if constexpr (!Q8) {
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const int r = 2 * c + (t & 1) + 8 * (t >> 1);
-                if constexpr (D == 128) {
-                    const uint4 w = lds128(vt + r * F::RB + v_chunk<D, Q8>(r, g) * 16);
-                    wv[t][0] = w.x, wv[t][1] = w.y, wv[t][W - 2] = w.z, wv[t][W - 1] = w.w;
-                } else {
-                    const uint32_t ad = vt + r * F::RB + v_chunk<D, Q8>(r, g >> 1) * 16 + (g & 1) * 8;
-                    wv[t][0] = lds32(ad), wv[t][1] = lds32(ad + 4);
+                for (int n = 0; n < NB; n += 2) {
+                    uint32_t v4[4];
+                    const int r = (lane & 7) + 8 * ((lane >> 3) & 1);
+                    ldsm4t(v4, vf + r * F::RB + v_chunk<D, Q8>(r, n + (lane >> 4)) * 16);
+                    mma16(o[n], pa[f], v4[0], v4[1]);
+                    mma16(o[n + 1], pa[f], v4[2], v4[3]);
+                }
+            } else {
+                // Block n, column g: element g * NB + n, so that a lane's elements of
+                // a value are consecutive bytes.
+                constexpr int W = D / 32;  // 32-bit words per lane and value
+                uint32_t wv[4][W];
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    const int r = 2 * c + (t & 1) + 8 * (t >> 1);
+                    if constexpr (D == 128) {
+                        const uint4 w = lds128(vf + r * F::RB + v_chunk<D, Q8>(r, g) * 16);
+                        wv[t][0] = w.x, wv[t][1] = w.y, wv[t][W - 2] = w.z, wv[t][W - 1] = w.w;
+                    } else {
+                        const uint32_t ad = vf + r * F::RB + v_chunk<D, Q8>(r, g >> 1) * 16 + (g & 1) * 8;
+                        wv[t][0] = lds32(ad), wv[t][1] = lds32(ad + 4);
+                    }
+#pragma unroll
+                    for (int w = 0; w < W; ++w) wv[t][w] ^= 0x80808080u;
                 }
 #pragma unroll
-                for (int w = 0; w < W; ++w) wv[t][w] ^= 0x80808080u;
-            }
+                for (int w = 0; w < W; ++w) {
 #pragma unroll
-            for (int w = 0; w < W; ++w) {
-                uint32_t bq[2][2];
-#pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    const uint32_t sel = hf ? 0x7362u : 0x5140u;
-                    bq[0][0] = __byte_perm(wv[0][w], wv[1][w], sel);
-                    bq[1][0] = __byte_perm(wv[2][w], wv[3][w], sel);
-                    mma16(o[4 * w + 2 * hf], pa, codes_fp16(bq[0][0], 0x4140), codes_fp16(bq[1][0], 0x4140));
-                    mma16(o[4 * w + 2 * hf + 1], pa, codes_fp16(bq[0][0], 0x4342), codes_fp16(bq[1][0], 0x4342));
+                    for (int hf = 0; hf < 2; ++hf) {
+                        const uint32_t sel = hf ? 0x7362u : 0x5140u;
+                        const uint32_t b0 = __byte_perm(wv[0][w], wv[1][w], sel);
+                        const uint32_t b1 = __byte_perm(wv[2][w], wv[3][w], sel);
+                        mma16(o[4 * w + 2 * hf], pa[f], codes_fp16(b0, 0x4140), codes_fp16(b1, 0x4140));
+                        mma16(o[4 * w + 2 * hf + 1], pa[f], codes_fp16(b0, 0x4342), codes_fp16(b1, 0x4342));
+                    }
                 }
             }
         }
@@ -564,9 +605,9 @@ __global__ void __launch_bounds__(kWarps * 32, 2) b200q_attn_few_kernel(const At
 }
 
 template <int D, bool PREC, bool Q8>
-int launch_few(const AttnArgs& a0, int max_rows, int max_kv, cudaStream_t st) {
+int launch_few(const AttnArgs& a0, int max_rows, int max_kv, int sms, cudaStream_t st) {
     using F = Few<D, PREC, Q8>;
-    static_assert(F::kTotal <= 113 * 1024, "two CTAs per SM");
+    static_assert(F::kTotal <= 226 * 1024 / kCtasPerSm<D, Q8> - 1024, "resident CTAs");
     AttnArgs a = a0;
     a.row_blocks = (max_rows + F::R - 1) / F::R;
     static std::mutex mu;
@@ -578,16 +619,22 @@ int launch_few(const AttnArgs& a0, int max_rows, int max_kv, cudaStream_t st) {
         const uint64_t bit = dev < 64 ? 1ull << dev : 0;
         if (!(done & bit)) {
             if (cudaFuncSetAttribute(b200q_attn_few_kernel<D, PREC, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     F::kTotal) != cudaSuccess)
+                                     F::kTotal) != cudaSuccess ||
+                cudaFuncSetAttribute(b200q_attn_few_kernel<D, PREC, Q8>, cudaFuncAttributeNonPortableClusterSizeAllowed,
+                                     1) != cudaSuccess)
                 return B200Q_ECUDA;
             done |= bit;
         }
     }
     const long long units = static_cast<long long>(a.r.batch) * a.kv.n_kv * a.row_blocks;
-    // CTAs per block of rows: enough for about four waves of two CTAs per SM
-    // (ragged lengths even out over them), at least four tiles per warp.
+    // CTAs per block of rows: as many as one wave holds while the blocks leave
+    // SMs idle, two where they fill more than half a wave (ragged lengths even out
+    // over the halves), and 32 positions a warp at least. Measured at 4 x 8 rows of
+    // 2000 positions: 17 us for one wave, 24 for two; 64 sequences of 100-8000: 191,
+    // 175, 186 us for 1, 2, 4.
+    const long long slots = static_cast<long long>(sms) * kCtasPerSm<D, Q8>;
     int c = 1;
-    while (c < kMaxCluster && units * c < 1184 && max_kv > c * 2 * kWarps * kTile * 2) c *= 2;
+    while (c < kMaxCluster && (units * c * 2 <= slots || c == 1) && max_kv > c * 2 * kWarps * 32) c *= 2;
     if (units * c > 0x7fffffffll) return B200Q_ESHAPE;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(units * c));
@@ -610,10 +657,10 @@ int launch_few(const AttnArgs& a0, int max_rows, int max_kv, cudaStream_t st) {
 
 }  // namespace
 
-int launch_attn_few(const AttnArgs& a, int hd, bool fp32, bool q8, int max_rows, int max_kv, cudaStream_t st) {
+int launch_attn_few(const AttnArgs& a, int hd, bool fp32, bool q8, int max_rows, int max_kv, int sms, cudaStream_t st) {
 #define B200Q_FEW(D)                                                                                       \
-    (fp32 ? (q8 ? launch_few<D, true, true>(a, max_rows, max_kv, st) : launch_few<D, true, false>(a, max_rows, max_kv, st)) \
-          : (q8 ? launch_few<D, false, true>(a, max_rows, max_kv, st) : launch_few<D, false, false>(a, max_rows, max_kv, st)))
+    (fp32 ? (q8 ? launch_few<D, true, true>(a, max_rows, max_kv, sms, st) : launch_few<D, true, false>(a, max_rows, max_kv, sms, st)) \
+          : (q8 ? launch_few<D, false, true>(a, max_rows, max_kv, sms, st) : launch_few<D, false, false>(a, max_rows, max_kv, sms, st)))
     return hd == 128 ? B200Q_FEW(128) : B200Q_FEW(64);
 #undef B200Q_FEW
 }

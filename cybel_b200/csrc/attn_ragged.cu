@@ -64,7 +64,8 @@ int launch_attention_paged(const void* q, int dtype, int n_tokens, int batch, co
     a.few_rows = kFewRows;
     const bool q8 = pkv.kv_mode == B200Q_KV_Q8;
     const long long most = static_cast<long long>(max_q_len < n_tokens ? max_q_len : n_tokens) * a.group;
-    rc = launch_attn_few(a, hd, dtype == B200Q_F32, q8, static_cast<int>(std::min<long long>(most, kFewRows)), max_kv_len, st);
+    rc = launch_attn_few(a, hd, dtype == B200Q_F32, q8, static_cast<int>(std::min<long long>(most, kFewRows)),
+                         max_kv_len, dev->num_sms, st);
     if (rc != B200Q_OK || most <= kFewRows) return rc;
     return launch_attn_tiles(a, hd, dtype == B200Q_F32, q8, static_cast<long long>(n_tokens) * a.group, max_kv_len,
                              dev->num_sms, st);

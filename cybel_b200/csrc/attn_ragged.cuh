@@ -162,7 +162,8 @@ __device__ __forceinline__ void store_out4(__half* p, float4 v) {
         make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
 
-int launch_attn_few(const AttnArgs& a, int hd, bool fp32, bool q8, int max_rows, int max_kv, cudaStream_t st);
+int launch_attn_few(const AttnArgs& a, int hd, bool fp32, bool q8, int max_rows, int max_kv, int sms,
+                    cudaStream_t st);
 
 int launch_attn_tiles(const AttnArgs& a, int hd, bool fp32, bool q8, long long total_rows, int max_kv, int sms,
                       cudaStream_t st);
