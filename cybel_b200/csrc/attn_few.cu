@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm<D, Q8>) b200q_attn_few
 #pragma unroll
                     for (int v = 0; v < NX; v += 2) {
                         const float2 z = mul2(make_float2(x[i2][v], x[i2][v + 1]), both(inv_cap));
-                        const float2 near = tanh_near(z);
+                        const float2 near = tanh_near<true>(z);
                         x[i2][v] = a.cap * (fabsf(z.x) > 1.0f ? tanh_far(z.x) : near.x);
                         x[i2][v + 1] = a.cap * (fabsf(z.y) > 1.0f ? tanh_far(z.y) : near.y);
                     }

@@ -39,16 +39,27 @@ __device__ __forceinline__ float rcp_fast(float x) {
     return y;
 }
 
-// tanh(z) for |z| <= 1: z P(z^2), P of degree 6 (minimax in the relative
-// error, by Remez's exchange: 2^-24).
+// tanh(z) = z P(z^2) near 0, P minimax in the relative error by Remez's
+// exchange: of degree 6 for |z| <= 1 (2^-24), or of degree 4 for |z| <= 0.7
+// (2^-21.6: a score of 30 moves by 1e-5, a weight by as much relatively, which
+// fp16 rounds by 2.4e-4).
+template <bool PREC>
 __device__ __forceinline__ float2 tanh_near(float2 z) {
     const float2 u = mul2(z, z);
-    float2 p = fma2(u, both(1.041022634e-03f), both(-6.203379105e-03f));
-    p = fma2(p, u, both(2.028998042e-02f));
-    p = fma2(p, u, both(-5.345702957e-02f));
-    p = fma2(p, u, both(1.332520408e-01f));
-    p = fma2(p, u, both(-3.333283915e-01f));
-    p = fma2(p, u, both(9.999999502e-01f));
+    float2 p;
+    if constexpr (PREC) {
+        p = fma2(u, both(1.041022634e-03f), both(-6.203379105e-03f));
+        p = fma2(p, u, both(2.028998042e-02f));
+        p = fma2(p, u, both(-5.345702957e-02f));
+        p = fma2(p, u, both(1.332520408e-01f));
+        p = fma2(p, u, both(-3.333283915e-01f));
+        p = fma2(p, u, both(9.999999502e-01f));
+    } else {
+        p = fma2(u, both(1.377371058e-02f), both(-5.083623594e-02f));
+        p = fma2(p, u, both(1.328111259e-01f));
+        p = fma2(p, u, both(-3.333021290e-01f));
+        p = fma2(p, u, both(9.999996973e-01f));
+    }
     return mul2(p, z);
 }
 // tanh(z) as 1 - 2 / (e^2z + 1) from two approximate instructions: off by 2^-22

@@ -150,7 +150,7 @@ struct Waiter {
     volatile uint32_t* dead;
     volatile int* status;
     __device__ __forceinline__ bool operator()(uint32_t bar, uint32_t parity) const {
-        return mbar_try_wait(bar, parity) || wait_slow(bar, parity, dead, status);
+        return mbar_test_wait(bar, parity) || mbar_try_wait(bar, parity) || wait_slow(bar, parity, dead, status);
     }
 };
 
@@ -466,9 +466,18 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
                 __syncwarp();
                 if (lane == 0) mbar_arrive(kvfull(x));
             };
+            // Waits for room before item x. Where there is none yet, what is on its way
+            // is handed over first: the room may depend on it.
+            int handed = 0;  // items finished
+            auto room = [&](uint32_t bar, uint32_t parity, int x) {
+                if (__all_sync(0xffffffffu, mbar_test_wait(bar, parity))) return true;
+                cp_async_wait<0>();
+                while (handed < x) finish(handed++);
+                ok = __all_sync(0xffffffffu, wait(bar, parity));
+                return ok;
+            };
             // Shared offsets of this thread's copies within the warp's 32 rows: they
             // repeat every 8 rows, up to the rows themselves.
-            int handed = 0;  // items finished
             constexpr int PAT = 8 / RPI;
             uint32_t pat[PAT];
 #pragma unroll
@@ -476,21 +485,14 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
             for (int i = 0; i < n && ok; ++i) {
                 const uint32_t row = ahead;
                 ahead = look(i + 1);
-                ok = __all_sync(0xffffffffu, wait(mempty(i), ((i / kMeta) & 1) ^ 1));
-                if (!ok) break;
+                if (!room(mempty(i), ((i / kMeta) & 1) ^ 1, 2 * i)) break;
                 put_meta(i, row);
                 // The warp's 32 rows one after the other in one page, as nearly always?
                 const uint32_t row0 = __shfl_sync(0xffffffffu, row, 0);
                 const bool run = __all_sync(0xffffffffu, row != kNoRow && row == row0 + lane);
                 for (int part = 0; part < 2; ++part) {
                     const int x = 2 * i + part;
-                    if (!__all_sync(0xffffffffu, mbar_test_wait(kvempty(x), ((x / NS) & 1) ^ 1))) {
-                        // the ring is full: hand over what is on its way first
-                        cp_async_wait<0>();
-                        while (handed < x) finish(handed++);
-                        ok = __all_sync(0xffffffffu, wait(kvempty(x), ((x / NS) & 1) ^ 1));
-                        if (!ok) break;
-                    }
+                    if (!room(kvempty(x), ((x / NS) & 1) ^ 1, x)) break;
                     const uint32_t slot = sbase + S::kRing + (x % NS) * S::kMat;
                     const uint8_t* src = static_cast<const uint8_t*>(part ? a.kv.v : a.kv.k) + (lane % CH) * 16;
                     if (run) {
@@ -668,7 +670,8 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
         }
         const bool shaped = a.cap > 0.0f || a.slopes != nullptr;
         const float inv_cap = a.cap > 0.0f ? 1.0f / a.cap : 0.0f;
-        const float to_log2 = shaped ? 1.0f : mult * kLog2e;  // factor left for the exponent
+        // Factor left for the exponent: of a raw score, of tanh (cap alone), or none.
+        const float to_log2 = !shaped ? mult * kLog2e : (a.slopes ? 1.0f : a.cap * kLog2e);
         const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
         const uint32_t ts = tmem + lanes + t * kRows, to = tmem + lanes + kO + t * D;
         const Steps mine(sight, list, i0, job.lo[t], job.hi[t]);
@@ -752,14 +755,17 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
 #pragma unroll
                         for (int u = 0; u < 4; ++u)
                             far[u] = max3(far[u], fabsf(x[c + 2 * u]), fabsf(x[c + 2 * u + 1]));
-                    const float f2 = a.cap * kLog2e;
-                    if (__any_sync(0xffffffffu, fmaxf(fmaxf(far[0], far[1]), fmaxf(far[2], far[3])) > 1.0f)) {
+                    if (__any_sync(0xffffffffu, fmaxf(fmaxf(far[0], far[1]), fmaxf(far[2], far[3])) > (PREC ? 1.0f : 0.7f))) {
 #pragma unroll
-                        for (int c = 0; c < kRows; ++c) x[c] = f2 * tanh_far(x[c]);
+                        for (int c = 0; c < kRows; ++c) x[c] = tanh_far(x[c]);
                     } else {
 #pragma unroll
+                        for (int c = 0; c < kRows; c += 2) put2(x + c, tanh_near<PREC>(make_float2(x[c], x[c + 1])));
+                    }
+                    if (a.slopes) {
+#pragma unroll
                         for (int c = 0; c < kRows; c += 2)
-                            put2(x + c, mul2(tanh_near(make_float2(x[c], x[c + 1])), both(f2)));
+                            put2(x + c, mul2(make_float2(x[c], x[c + 1]), both(a.cap * kLog2e)));
                     }
                 }
                 if (a.slopes) {
@@ -815,6 +821,7 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
             float2 s2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
             for (int quarter = 0; quarter < 4; ++quarter) {
+                if (quarter == 3 && lane == 0) mbar_arrive(next_turn);  // its first loads run under this one's tail
                 uint32_t hi16[16], lo16[16];
                 float4 v4;
 #pragma unroll
@@ -842,7 +849,6 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
                 tmem_st16(ts + quarter * 16, hi16);
                 if constexpr (PREC) tmem_st16(ts + 64 + quarter * 16, lo16);
             }
-            if (lane == 0) mbar_arrive(next_turn);
             const float2 st = add2(s2[0], s2[1]);
             l += st.x + st.y;
             tmem_wait_st();
