@@ -231,61 +231,7 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
     volatile uint32_t* any_bad = reinterpret_cast<volatile uint32_t*>(smem + S::kJob + 116);  // any of bad_bits
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t C = cluster_size(), rank = cluster_rank();
-    griddep_launch_dependents();
-    griddep_wait();
-
-    // ---- which rows: blocks of 256 rows of the sequences with more than
-    // few_rows rows, the later blocks of a sequence (more positions) first
-    const int cluster = blockIdx.x / C;
-    if (warp == 0) {
-        auto blocks = [&](int b) {
-            if (b >= a.r.batch) return 0;
-            const int2 rr = seq_rows(a.r, b);
-            const int rows = (rr.y - rr.x) * a.group;
-            return rows > a.few_rows ? (rows + kCtaRows - 1) / kCtaRows : 0;
-        };
-        int total = 0;
-        for (int b0 = 0; b0 < a.r.batch; b0 += 32) total += blocks(b0 + lane);
-        total = __reduce_add_sync(0xffffffffu, total);
-        const int kvh = cluster % a.kv.n_kv;
-        int x = total - 1 - cluster / a.kv.n_kv;
-        if (lane == 0) {
-            job_s->live = x >= 0;
-            *dead = 0;
-            *any_bad = 0;
-        }
-        for (int b0 = 0; b0 < a.r.batch && x >= 0; b0 += 32) {
-            const int mine = blocks(b0 + lane);
-            int upto = mine;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= o) upto += y;
-            }
-            if (x < upto && x >= upto - mine) {
-                Job j;
-                j.live = 1;
-                const int2 rr = seq_rows(a.r, b0 + lane);
-                j.b = b0 + lane;
-                j.kvh = kvh;
-                j.rows = (rr.y - rr.x) * a.group;
-                j.row0 = (x - (upto - mine)) * kCtaRows;
-                j.first_tok = rr.x;
-                j.sight = sight_of(a, j.b);
-                j.p0 = j.sight.n - (rr.y - rr.x);
-                for (int t = 0; t < kTiles; ++t) {
-                    const int r0 = j.row0 + t * kRows, r1 = min(r0 + kRows, j.rows) - 1;
-                    j.lo[t] = j.p0 + r0 / a.group;
-                    j.hi[t] = r1 >= r0 ? j.p0 + r1 / a.group : -1;
-                    if (r1 < r0) j.lo[t] = 0;
-                }
-                *job_s = j;
-            }
-            const int got = __shfl_sync(0xffffffffu, upto, 31);
-            x = x < got ? -1 : x - got;
-        }
-    }
-    for (int i = threadIdx.x; i < kBadWords; i += kThreads) reinterpret_cast<uint32_t*>(smem + S::kBad)[i] = 0;
+    // What needs no input comes before the wait for the kernel ahead.
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
     const uint32_t bar0 = smem_addr(bars);
     auto kvfull = [&](int i) { return bar0 + 8u * (i % NS); };
@@ -316,16 +262,77 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
         mbar_init(done, kTiles);
         fence_mbar_init();
     }
-    __syncthreads();
-    if (!job_s->live) return;  // the whole cluster
     if (warp == 12) {
         tmem_alloc(smem_addr(tmem_holder), 512);
         tmem_relinquish();
     }
+    griddep_launch_dependents();
+    griddep_wait();
+
+    // ---- which rows: blocks of 256 rows of the sequences with more than
+    // few_rows rows, the later blocks of a sequence (more positions) first
+    const int cluster = blockIdx.x / C;
+    if (warp == 0) {
+        // the first 32 sequences' entries in one trip to memory
+        const int b_lane = min(lane, a.r.batch - 1);
+        const int2 rr_lane = seq_rows(a.r, b_lane);
+        const Sight sight_lane = sight_of(a, b_lane);
+        auto blocks = [&](int b) {
+            if (b >= a.r.batch) return 0;
+            const int2 rr = b < 32 ? rr_lane : seq_rows(a.r, b);
+            const int rows = (rr.y - rr.x) * a.group;
+            return rows > a.few_rows ? (rows + kCtaRows - 1) / kCtaRows : 0;
+        };
+        int total = 0;
+        for (int b0 = 0; b0 < a.r.batch; b0 += 32) total += blocks(b0 + lane);
+        total = __reduce_add_sync(0xffffffffu, total);
+        const int kvh = cluster % a.kv.n_kv;
+        int x = total - 1 - cluster / a.kv.n_kv;
+        if (lane == 0) {
+            job_s->live = x >= 0;
+            *dead = 0;
+            *any_bad = 0;
+        }
+        for (int b0 = 0; b0 < a.r.batch && x >= 0; b0 += 32) {
+            const int mine = blocks(b0 + lane);
+            int upto = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += y;
+            }
+            if (x < upto && x >= upto - mine) {
+                Job j;
+                j.live = 1;
+                const int2 rr = b0 == 0 ? rr_lane : seq_rows(a.r, b0 + lane);
+                j.b = b0 + lane;
+                j.kvh = kvh;
+                j.rows = (rr.y - rr.x) * a.group;
+                j.row0 = (x - (upto - mine)) * kCtaRows;
+                j.first_tok = rr.x;
+                j.sight = b0 == 0 ? sight_lane : sight_of(a, j.b);
+                j.p0 = j.sight.n - (rr.y - rr.x);
+                for (int t = 0; t < kTiles; ++t) {
+                    const int r0 = j.row0 + t * kRows, r1 = min(r0 + kRows, j.rows) - 1;
+                    j.lo[t] = j.p0 + div_by(r0, a.group_mul, a.group_shift);
+                    j.hi[t] = r1 >= r0 ? j.p0 + div_by(r1, a.group_mul, a.group_shift) : -1;
+                    if (r1 < r0) j.lo[t] = 0;
+                }
+                *job_s = j;
+            }
+            const int got = __shfl_sync(0xffffffffu, upto, 31);
+            x = x < got ? -1 : x - got;
+        }
+    }
+    for (int i = threadIdx.x; i < kBadWords; i += kThreads) reinterpret_cast<uint32_t*>(smem + S::kBad)[i] = 0;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_holder;
+    if (!job_s->live) {  // the whole cluster
+        if (warp == 12) tmem_dealloc(tmem, 512);
+        return;
+    }
     const Job& job = *job_s;
     const Sight sight = job.sight;
     const int lo = job.lo[0], hi = max(job.hi[0], job.hi[1]);
@@ -609,13 +616,11 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
             // Q of the warp's 32 rows, a row (fp32) or two (fp16) per load: fp16 as it
             // is, fp32 as two parts of q 2^10 / E, E a power of two above the row
             const uint32_t dst = sbase + t * S::kParts * S::kMat;
-            const int w32 = (warp & 3) * 32, first_row = job.row0 + t * kRows + w32;
-            auto source = [&](int r) {  // row first_row + r, NULL past the sequence
-                const int rw = first_row + r;
-                const int tk = div_by(rw, a.group_mul, a.group_shift);
-                return rw < job.rows ? static_cast<const T*>(a.q) + (job.first_tok + tk) * a.q_stride +
-                                           (job.kvh * a.group + rw - tk * a.group) * D
-                                     : nullptr;
+            const int w32 = (warp & 3) * 32;
+            const long long mine = have ? (job.first_tok + tok) * a.q_stride + head * D : -1;  // of lane's row
+            auto source = [&](int r) {  // row r of the warp's, NULL past the sequence
+                const long long off = __shfl_sync(0xffffffffu, mine, r);
+                return off >= 0 ? static_cast<const T*>(a.q) + off : nullptr;
             };
             if constexpr (!PREC) {
                 constexpr int CH = D / 8, RPI = 32 / CH, NI = 32 / RPI;
@@ -925,14 +930,14 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
             __syncwarp();
             constexpr int CH = kRowBytes / 16, RPI = 32 / CH, NI = 32 / RPI;
             const int w32 = (warp & 3) * 32;
+            const long long to_out = have ? (job.first_tok + tok) * a.out_stride + head * D : -1;
 #pragma unroll 8
             for (int k = 0; k < NI; ++k) {
-                const int r = w32 + k * RPI + lane / CH, rw = job.row0 + t * kRows + r;
-                if (rw >= job.rows) continue;
+                const int r = w32 + k * RPI + lane / CH;
+                const long long off = __shfl_sync(0xffffffffu, to_out, k * RPI + lane / CH);
+                if (off < 0) continue;
                 const uint4 v = lds128(sbase + t * S::kParts * S::kMat + r * kRowBytes + (((lane % CH) ^ (r & 7)) << 4));
-                const int tk = div_by(rw, a.group_mul, a.group_shift);
-                *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (job.first_tok + tk) * a.out_stride +
-                                          (job.kvh * a.group + rw - tk * a.group) * D + (lane % CH) * (16 / sizeof(T))) = v;
+                *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + off + (lane % CH) * (16 / sizeof(T))) = v;
             }
         }
         tc_fence_before();
