@@ -181,6 +181,7 @@ class DecodeStack:
         self.fused_norm = fused_norm
         self.fused_swiglu = fused_swiglu
         self._vbufs: dict = {}  # verify-pass buffers per row count
+        self._prompt = None     # prefill's view of the cache and rotary table
         self.dev = torch.device("cuda", device)
         self.lib = _native.lib()
         f32 = dict(dtype=torch.float32, device=self.dev)
@@ -313,6 +314,82 @@ class DecodeStack:
 
     def set_token(self, token: int) -> None:
         self.token.fill_(int(token))
+
+    # -- a prompt ------------------------------------------------------------------
+    def prefill(self, tokens, pos0: int = 0, chunk: int = 512):
+        """Feed a prompt at positions pos0, pos0 + 1, ... through the stack,
+        `chunk` tokens a pass, and leave the last token's logits in
+        ``self.logits`` (returned), as len(tokens) calls of ``step`` would: the
+        linears run over the rows of a pass (b200q_matmul_ex: the tcgen05 tile
+        kernel for Q4_K), its keys and values are appended and its rows attend
+        over the cache in two launches per layer
+        (b200q_rope_append_paged, b200q_attention_paged), and only the last
+        row meets the LM head. Works on any of the stack's caches. ``tokens``:
+        integers, or an integer tensor."""
+        import torch
+
+        from .kv_cache import PagedKVCache
+        from .paged_attention import RaggedBatch, RopeTable
+
+        n = len(tokens)
+        if n <= 0 or chunk <= 0:
+            raise ValueError("no tokens to prefill")
+        if pos0 < 0 or pos0 + n > self.max_ctx:
+            raise ValueError("positions outside the KV cache")
+        s, L = self.shape, self.lib
+        if self._prompt is None:
+            cache = self.kv_cache
+            if cache is None:
+                cache = PagedKVCache.over_contiguous(self.k_cache, self.v_cache)
+            self._prompt = (cache, RopeTable(s.head_dim, s.rope_theta, device=self.dev.index))
+        cache, rope = self._prompt
+        ids = tokens if isinstance(tokens, torch.Tensor) else torch.tensor([int(t) for t in tokens])
+        ids = ids.to(device=self.dev, dtype=torch.int32)
+        if self.kv_cache is not None:
+            cache.ensure(pos0, pos0 + n - 1)
+        act, W = self.act_mode, _native.WEIGHTS_STATIC | _native.TILE_FROM_2
+        h, kv, hd, f = s.hidden, s.kv_dim, s.head_dim, s.ffn
+        z = (lambda *shape: torch.empty(shape, dtype=torch.float32, device=self.dev))
+        rows = min(n, chunk)
+        B = dict(x=z(rows, h), hn=z(rows, h), qkv=z(rows, h + 2 * kv), q=z(rows, h), att=z(rows, h), o=z(rows, h),
+                 gu=z(rows, 2 * f), sw=z(rows, f), d=z(rows, h))
+        P = {name: t.data_ptr() for name, t in B.items()}
+        st = torch.cuda.current_stream(self.dev).cuda_stream
+        for c0 in range(0, n, chunk):
+            m = min(chunk, n - c0)
+            last = c0 + m == n
+            batch = RaggedBatch([m], [pos0 + c0 + m], device=self.dev.index)
+            qkv = B["qkv"][:m]
+            q = qkv[:, :h].view(m, s.heads, hd)
+            k = qkv[:, h:h + kv].view(m, s.kv_heads, hd)
+            v = qkv[:, h + kv:].view(m, s.kv_heads, hd)
+            qr, att = B["q"][:m].view(m, s.heads, hd), B["att"][:m].view(m, s.heads, hd)
+
+            def lin(mat, n_out, x, y, k_in, rows=m):
+                self._check(L.b200q_matmul_ex(mat.qtype, act, x, mat.ptr, y, rows, k_in, n_out, W, st), "prefill linear")
+
+            self._check(L.b200q_dequantize_rows(s.embedding_qtype, self.embed.ptr, ids[c0:].data_ptr(), m, P["x"], h,
+                                                s.vocab, st), "embedding")
+            delta = None
+            for li, lay in enumerate(self.layers):
+                self._check(L.b200q_add_rmsnorm(P["x"], delta, lay.attn_norm.data_ptr(), P["hn"], h, m, s.eps, st),
+                            "attn norm")
+                lin(lay.wqkv, h + 2 * kv, P["hn"], P["qkv"], h)
+                cache.append(li, k, v, batch, rope=rope, q=q, q_out=qr)
+                cache.attend(li, qr, batch, out=att)
+                lin(lay.wo, h, P["att"], P["o"], h)
+                self._check(L.b200q_add_rmsnorm(P["x"], P["o"], lay.ffn_norm.data_ptr(), P["hn"], h, m, s.eps, st),
+                            "ffn norm")
+                lin(lay.w_gu, 2 * f, P["hn"], P["gu"], h)
+                self._check(L.b200q_swiglu_rows(P["gu"], P["sw"], m, f, st), "swiglu")
+                lin(lay.w_down, h, P["sw"], P["d"], f)
+                delta = P["d"]
+            if last:
+                x_last, d_last = P["x"] + 4 * h * (m - 1), delta + 4 * h * (m - 1)
+                self._check(L.b200q_add_rmsnorm(x_last, d_last, self.out_norm.data_ptr(), P["hn"], h, 1, s.eps, st),
+                            "output norm")
+                lin(self.head, s.vocab, P["hn"], self.logits.data_ptr(), h, rows=1)
+        return self.logits
 
     # -- several tokens in one pass ---------------------------------------------
     def _verify_buffers(self, m: int) -> dict:

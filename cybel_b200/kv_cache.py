@@ -99,6 +99,28 @@ class PagedKVCache:
         self.table = torch.from_numpy(self.table_host).to(self.dev)
         self._free = list(range(self.n_slots - 1, -1, -1))  # pop() hands out slot 0 first
 
+    @classmethod
+    def over_contiguous(cls, k, v) -> "PagedKVCache":
+        """A view of contiguous fp16 caches [layers][kv_heads][max_ctx]
+        [head_dim] of one sequence as pages: one page of max_ctx positions per
+        layer, every page assigned. ``append`` and ``attend`` then work on the
+        contiguous cache itself."""
+        import torch
+
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != torch.float16 or v.dtype != torch.float16:
+            raise ValueError("k and v must be fp16 [layers][kv_heads][max_ctx][head_dim]")
+        if not (k.is_contiguous() and v.is_contiguous()) or k.shape[3] not in HEAD_DIMS:
+            raise ValueError("k and v must be contiguous, heads of 64 or 128")
+        self = cls.__new__(cls)
+        self.layers, self.kv_heads, self.max_seq, self.head_dim = k.shape
+        self.batch, self.pages_per_seq, self.page_size, self.q8 = 1, 1, self.max_seq, False
+        self.n_slots, self.dev = self.layers, k.device
+        self.k, self.v, self.ks, self.vs = k, v, None, None
+        self.table_host = np.arange(self.layers, dtype=np.int32).reshape(self.layers, 1, 1)
+        self.table = torch.from_numpy(self.table_host).to(self.dev)
+        self._free = []
+        return self
+
     # -- page assignment -------------------------------------------------------
     @property
     def kv_mode(self) -> int:

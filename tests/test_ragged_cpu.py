@@ -134,3 +134,12 @@ def test_row_strides():
     assert _row_stride(torch.zeros(0, 3, 64), "x") == 192
     with pytest.raises(ValueError):
         _row_stride(torch.zeros(1, 3, 64).expand(4, 3, 64), "x")
+
+
+def test_over_contiguous():
+    k = torch.zeros(3, 2, 50, 64, dtype=torch.float16)
+    c = PagedKVCache.over_contiguous(k, torch.zeros_like(k))
+    assert c.table.tolist() == [[[0]], [[1]], [[2]]] and c.page_size == 50 and c.kv_mode == _native.KV_F16
+    for a, b in ((k, k[:2]), (k.float(), k.float()), (k.transpose(1, 2), k.transpose(1, 2)), (k[..., :32], k[..., :32])):
+        with pytest.raises(ValueError):
+            PagedKVCache.over_contiguous(a, b)

@@ -554,3 +554,111 @@ def test_two_streams_at_once():
                 o.append(c.attend(0, q, batch))
     _clean()
     assert all(torch.equal(x, want) for o in outs for x in o)
+
+
+def test_refused_calls_launch_nothing():
+    """Every refusal of the C entry points comes before a launch: the outputs
+    keep what they held."""
+    import torch
+
+    from cybel_b200 import _native
+    from cybel_b200.paged_attention import RopeTable
+
+    L = _native.lib()
+    st = torch.cuda.current_stream().cuda_stream
+    c, b = _cache([2, 3], [40, 50], 2, 128, 16, True, seed=1)
+    q = torch.randn(5, 4, 128, device="cuda")
+    out = torch.full_like(q, 3.0)
+    pos = torch.arange(5, dtype=torch.int32, device="cuda")
+    t = RopeTable(128)
+    k0 = c.k.clone()
+
+    def attend(**kw):
+        d = dict(q=q.data_ptr(), dtype=0, n=5, batch=2, cu=b.cu_q.data_ptr(), kl=b.kv_len.data_ptr(), mq=3, mk=50, h=4,
+                 kv=2, hd=128, qs=0, out=out.data_ptr(), os=0, scale=0.1, cap=0.0, sl=None, w=0, pre=None, mode=1,
+                 k=c.k.data_ptr(), v=c.v.data_ptr(), ks=c.ks.data_ptr(), vs=c.vs.data_ptr(), slots=c.n_slots, page=16,
+                 tab=c.table_ptr(0), pps=c.pages_per_seq) | kw
+        return L.b200q_attention_paged(*d.values(), st)
+
+    def append(**kw):
+        d = dict(q=q.data_ptr(), k=q.data_ptr(), v=q.data_ptr(), dtype=0, n=5, batch=2, cu=b.cu_q.data_ptr(),
+                 kl=b.kv_len.data_ptr(), h=4, kv=2, hd=128, qs=0, kvs=512, out=out.data_ptr(), os=0,
+                 turns=t.turns.data_ptr(), rot=128, layout=0, mag=1.0, mode=1, kp=c.k.data_ptr(), vp=c.v.data_ptr(),
+                 ks=c.ks.data_ptr(), vs=c.vs.data_ptr(), slots=c.n_slots, page=16, tab=c.table_ptr(0),
+                 pps=c.pages_per_seq) | kw
+        return L.b200q_rope_append_paged(*d.values(), st)
+
+    def rows(**kw):
+        d = dict(x=q.data_ptr(), out=out.data_ptr(), dtype=0, n=5, h=4, hd=128, xs=0, os=0, pos=pos.data_ptr(),
+                 turns=t.turns.data_ptr(), rot=128, layout=0, mag=1.0) | kw
+        return L.b200q_rope_rows(*d.values(), st)
+
+    inv, shape, align = -1, -3, -4
+    for fn, cases in (
+        (attend, [(dict(q=None), inv), (dict(out=None), inv), (dict(cu=None), inv), (dict(kl=None), inv),
+                  (dict(dtype=2), inv), (dict(batch=0), inv), (dict(n=-1), inv), (dict(scale=0.0), inv),
+                  (dict(scale=float("nan")), inv), (dict(cap=-1.0), inv), (dict(cap=float("inf")), inv),
+                  (dict(w=-1), inv), (dict(mode=2), inv), (dict(ks=None), inv), (dict(tab=None), inv),
+                  (dict(slots=0), inv), (dict(page=0), inv), (dict(h=5), shape), (dict(hd=96), shape),
+                  (dict(qs=511), shape), (dict(os=100), shape), (dict(page=2 ** 30, pps=2), shape),
+                  (dict(slots=2 ** 31 - 1), shape), (dict(q=q.data_ptr() + 4), align), (dict(qs=513), align),
+                  (dict(k=c.k.data_ptr() + 8), align), (dict(tab=c.table_ptr(0) + 2), align)]),
+        (append, [(dict(k=None), inv), (dict(v=None), inv), (dict(q=None), inv), (dict(dtype=7), inv),
+                  (dict(layout=2), inv), (dict(mode=-1), inv), (dict(vs=None), inv), (dict(turns=None), shape),
+                  (dict(rot=130), shape), (dict(rot=7), shape), (dict(kvs=255), shape), (dict(hd=256), shape),
+                  (dict(k=q.data_ptr() + 2), align), (dict(turns=t.turns.data_ptr() + 4), align)]),
+        (rows, [(dict(x=None), inv), (dict(pos=None), inv), (dict(turns=None), inv), (dict(dtype=3), inv),
+                (dict(h=0), inv), (dict(layout=5), inv), (dict(rot=0), shape), (dict(rot=129), shape),
+                (dict(hd=64), shape), (dict(xs=511), shape), (dict(x=q.data_ptr() + 2), align)]),
+    ):
+        for kw, want in cases:
+            assert fn(**kw) == want, (fn.__name__, kw)
+    torch.cuda.synchronize()
+    assert (out == 3).all() and torch.equal(c.k, k0)
+    assert attend(n=0) == 0 and append(n=0) == 0 and rows(n=0) == 0
+    assert rows() == 0 and attend() == 0
+    _clean()
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "fp16"])
+def test_attend_many_sequences_and_large_groups(dtype):
+    """More sequences than a warp's lanes, some long and some empty, and more
+    query heads per kv head than a tile of rows holds tokens for."""
+    import torch
+
+    ql = [(i * 7) % 5 if i % 11 else 70 for i in range(75)]
+    kl = [n + (i * 37) % 200 for i, n in enumerate(ql)]
+    for heads, kv in ((4, 2), (40, 1)):
+        c, batch = _cache(ql, kl, kv, 64, 32, False, seed=kv, poison=True)
+        q = torch.randn(batch.n_tokens, heads, 64, device="cuda").to(_dt(dtype))
+        out = c.attend(0, q, batch)
+        _clean()
+        _check_attend(c, 0, batch, q, out)
+
+
+def test_graph_with_a_split_and_changing_lengths():
+    """A captured call over both kernels replays with other lengths: a long
+    sequence's chunk shrinks to a single row and grows back."""
+    import torch
+
+    from cybel_b200.paged_attention import RaggedBatch
+
+    c, _ = _cache([1, 1], [4000, 300], 2, 128, 64, False, seed=8)
+    batch = RaggedBatch([100, 20], [4000, 300])
+    q = torch.randn(batch.n_tokens, 8, 128, device="cuda").half()
+    out = torch.empty_like(q)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        c.attend(0, q, batch, out=out)
+    torch.cuda.current_stream().wait_stream(s)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        c.attend(0, q, batch, out=out)
+    for ql, kl in (([100, 20], [4000, 300]), ([1, 0], [2100, 7]), ([0, 0], [5, 0]), ([7, 90], [3999, 299])):
+        batch.update(ql, kl)
+        out.fill_(2.0)
+        g.replay()
+        _clean()
+        _check_attend(c, 0, batch, q, out)
+        assert (out[sum(ql):] == 2).all()
