@@ -47,16 +47,18 @@ struct Few {
     static constexpr int kTile = RB == 256 ? 16 : 32;
     static constexpr int kScales = Q8 ? 2 * kTile * 4 : 0;  // the tile's key and value scales
     static constexpr int kStage = 2 * kTile * RB + kScales;
-    static constexpr int NS = RB == 128 ? 2 : 3;
+    static constexpr int NS = RB == 64 ? 3 : 2;
     static constexpr int kRing = NS * kStage;
     static constexpr int kPart = R * D * 4;               // a warp's output, in its ring after the loop
     static constexpr int kWarpBytes = kRing > kPart ? kRing : kPart;
     static constexpr int kTotal = kWarps * kWarpBytes + kWarps * R * 8 + R * 8;
 };
 
-// Resident CTAs per SM: rows of 256 bytes fill the shared memory with two.
-template <int D, bool Q8>
-constexpr int kCtasPerSm = (Q8 ? D : 2 * D) == 256 ? 2 : 3;
+// Resident CTAs per SM, which registers and rings are cut to: twelve warps with
+// one tile on its way each beat eight with two (64 sequences of 100-8000
+// positions in Q8 pages 148 -> 134 us, two of 60-120 thousand in fp16 pages 198
+// -> 156; four times eight rows of 2000 positions 17 -> 20).
+constexpr int kCtasPerSm = 3;
 
 __device__ __forceinline__ void ldsm4(uint32_t (&v)[4], uint32_t a) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -116,7 +118,7 @@ __device__ __forceinline__ int v_chunk(int r, int c) {
 }
 
 template <int D, bool PREC, bool Q8>
-__global__ void __launch_bounds__(kWarps * 32, kCtasPerSm<D, Q8>) b200q_attn_few_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) b200q_attn_few_kernel(const AttnArgs a) {
     using F = Few<D, PREC, Q8>;
     using T = typename std::conditional<PREC, float, __half>::type;
     constexpr int R = F::R, KS = D / 16, NB = D / 8, NS = F::NS, kTile = F::kTile;
@@ -140,6 +142,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm<D, Q8>) b200q_attn_few
     const int r0 = rb * R;
     if (rows > a.few_rows || r0 >= rows) return;  // the same for the whole cluster
     const Sight s = sight_of(a, b);
+    if (threadIdx.x == 0 && s.n > s.limit) flag_bad_page(a.kv);
     const int nr = min(R, rows - r0);
     const int p0 = s.n - (rr.y - rr.x);
     const int p_lo = p0 + r0 / a.group, p_hi = p0 + (r0 + nr - 1) / a.group;
@@ -218,7 +221,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm<D, Q8>) b200q_attn_few
     const int stride = kWarps * static_cast<int>(C);
     const int first = static_cast<int>(rank) * kWarps + warp;
     const int n_mine = p_hi < 0 || tiles.count <= first ? 0 : (tiles.count - first + stride - 1) / stride;
-    const int hi_seen = max(p_hi, s.pre - 1), lo_seen = s.first(max(p_lo, 0));
+    const int hi_seen = s.last(p_hi), lo_seen = s.first(max(p_lo, 0));
 
     // Position lane % kTile of my tile i: its pool row, if some row of the block sees it.
     auto look = [&](int i) -> uint32_t {
@@ -607,7 +610,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm<D, Q8>) b200q_attn_few
 template <int D, bool PREC, bool Q8>
 int launch_few(const AttnArgs& a0, int max_rows, int max_kv, int sms, cudaStream_t st) {
     using F = Few<D, PREC, Q8>;
-    static_assert(F::kTotal <= 226 * 1024 / kCtasPerSm<D, Q8> - 1024, "resident CTAs");
+    static_assert(F::kTotal <= 226 * 1024 / kCtasPerSm - 1024, "resident CTAs");
     AttnArgs a = a0;
     a.row_blocks = (max_rows + F::R - 1) / F::R;
     static std::mutex mu;
@@ -632,7 +635,7 @@ int launch_few(const AttnArgs& a0, int max_rows, int max_kv, int sms, cudaStream
     // over the halves), and 32 positions a warp at least. Measured at 4 x 8 rows of
     // 2000 positions: 17 us for one wave, 24 for two; 64 sequences of 100-8000: 191,
     // 175, 186 us for 1, 2, 4.
-    const long long slots = static_cast<long long>(sms) * kCtasPerSm<D, Q8>;
+    const long long slots = static_cast<long long>(sms) * kCtasPerSm;
     int c = 1;
     while (c < kMaxCluster && (units * c * 2 <= slots || c == 1) && max_kv > c * 2 * kWarps * 32) c *= 2;
     if (units * c > 0x7fffffffll) return B200Q_ESHAPE;
@@ -652,7 +655,14 @@ int launch_few(const AttnArgs& a0, int max_rows, int max_kv, int sms, cudaStream
         attr[1].val.programmaticStreamSerializationAllowed = 1;
         cfg.numAttrs = 2;
     }
-    return cudaLaunchKernelEx(&cfg, b200q_attn_few_kernel<D, PREC, Q8>, a) == cudaSuccess ? B200Q_OK : B200Q_ECUDA;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, b200q_attn_few_kernel<D, PREC, Q8>, a);
+    if (e != cudaSuccess && c > 8) {  // no room for clusters of 16 (a partitioned device): the portable size
+        cudaGetLastError();
+        attr[0].val.clusterDim.x = 8;
+        cfg.gridDim.x = static_cast<unsigned>(units * 8);
+        e = cudaLaunchKernelEx(&cfg, b200q_attn_few_kernel<D, PREC, Q8>, a);
+    }
+    return e == cudaSuccess ? B200Q_OK : B200Q_ECUDA;
 }
 
 }  // namespace

@@ -40,8 +40,8 @@ __device__ __forceinline__ float rcp_fast(float x) {
 }
 
 // tanh(z) = z P(z^2) near 0, P minimax in the relative error by Remez's
-// exchange: of degree 6 for |z| <= 1 (2^-24), or of degree 4 for |z| <= 0.7
-// (2^-21.6: a score of 30 moves by 1e-5, a weight by as much relatively, which
+// exchange: of degree 6 for |z| <= 1 (2^-24), or of degree 3 for |z| <= 1/2
+// (2^-20.8: a score of 15 moves by 8e-6, a weight by as much relatively, which
 // fp16 rounds by 2.4e-4).
 template <bool PREC>
 __device__ __forceinline__ float2 tanh_near(float2 z) {
@@ -55,10 +55,9 @@ __device__ __forceinline__ float2 tanh_near(float2 z) {
         p = fma2(p, u, both(-3.333283915e-01f));
         p = fma2(p, u, both(9.999999502e-01f));
     } else {
-        p = fma2(u, both(1.377371058e-02f), both(-5.083623594e-02f));
-        p = fma2(p, u, both(1.328111259e-01f));
-        p = fma2(p, u, both(-3.333021290e-01f));
-        p = fma2(p, u, both(9.999996973e-01f));
+        p = fma2(u, both(-4.440222613e-02f), both(1.319029660e-01f));
+        p = fma2(p, u, both(-3.332631794e-01f));
+        p = fma2(p, u, both(9.999994558e-01f));
     }
     return mul2(p, z);
 }
@@ -78,8 +77,11 @@ __device__ __forceinline__ float pow2_above(float x) {
 // the row at position i, [i - window + 1, i]; n positions in all.
 struct Sight {
     int n, pre, window;
+    int limit;  // positions that the page table reaches, n at most
     // First position of the range that the row at position i sees by itself.
     __device__ __forceinline__ int first(int i) const { return window > 0 ? max(0, i - window + 1) : 0; }
+    // Last position that rows up to position hi see and the table reaches.
+    __device__ __forceinline__ int last(int hi) const { return min(max(hi, pre - 1), limit - 1); }
     __device__ __forceinline__ bool sees(int i, int j) const { return j < pre || (j <= i && j >= first(i)); }
     // Whether every row at lo .. hi sees all of j0 .. j1.
     __device__ __forceinline__ bool all(int lo, int hi, int j0, int j1) const {
@@ -90,7 +92,8 @@ struct Sight {
 __device__ __forceinline__ Sight sight_of(const AttnArgs& a, int b) {
     Sight s;
     s.n = a.r.kv_len[b];
-    s.pre = a.prefix ? min(max(a.prefix[b], 0), max(s.n, 0)) : 0;
+    s.limit = min(max(s.n, 0), a.kv.pages_per_seq * a.kv.page);
+    s.pre = a.prefix ? min(max(a.prefix[b], 0), s.limit) : 0;
     s.window = a.window;
     return s;
 }
@@ -103,8 +106,8 @@ struct TileList {
     __device__ __forceinline__ TileList(const Sight& s, int lo, int hi) {
         from = s.first(max(lo, 0)) / T;
         before = min((s.pre + T - 1) / T, from);
-        const int last = max(hi, s.pre - 1);
-        count = last < 0 ? 0 : before + last / T - from + 1;
+        const int last = s.last(hi);
+        count = before + max(0, last / T - from + (last >= 0));
     }
     __device__ __forceinline__ int at(int i) const { return (i < before ? i : from + i - before) * T; }
 };

@@ -102,7 +102,7 @@ struct Steps {
         const bool any = hi >= max(lo, 0);
         prefix = any ? (s.pre + kRows - 1) / kRows - i0 : 0;
         from = list.before + max(s.first(max(lo, 0)) / kRows - list.from, 0) - i0;
-        to = any ? list.before + max(hi, s.pre - 1) / kRows - list.from - i0 : -1;
+        to = any && s.last(hi) >= 0 ? list.before + s.last(hi) / kRows - list.from - i0 : -1;
     }
     __device__ __forceinline__ bool has(int i) const { return i < prefix || (i >= from && i <= to); }
 };
@@ -338,6 +338,7 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
     const int lo = job.lo[0], hi = max(job.hi[0], job.hi[1]);
     const TileList<kRows> list(sight, lo, hi);
     const int n_all = hi < 0 ? 0 : list.count;
+    if (threadIdx.x == 0 && sight.n > sight.limit) flag_bad_page(a.kv);
     const int i0 = static_cast<int>(static_cast<long long>(n_all) * rank / C);
     const int n = static_cast<int>(static_cast<long long>(n_all) * (rank + 1) / C) - i0;  // steps of this CTA
     const Waiter wait{dead, a.kv.status};
@@ -409,7 +410,7 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(loader_regs(Q8)));
         // ---------------- loader ----------------
         const int r = threadIdx.x - 256, w = warp - 8;
-        const int hi_seen = max(hi, sight.pre - 1), lo_seen = sight.first(max(lo, 0));
+        const int hi_seen = sight.last(hi), lo_seen = sight.first(max(lo, 0));
         auto look = [&](int i) -> uint32_t {
             if (i >= n) return kNoRow;
             const int j = pos_of(i) + r;
@@ -448,20 +449,33 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
         if constexpr (!Q8) {
             constexpr int CH = D / 8, RPI = 32 / CH, NI = 32 / RPI;  // chunks per row, rows per copy, copies
             constexpr int LA = NS >= 5 ? 2 : 1;                      // items in flight behind the newest
+            // Shared offsets of this thread's copies within the warp's 32 rows: they
+            // repeat every 8 rows, up to the rows themselves.
+            constexpr int PAT = 8 / RPI;
+            uint32_t pat[PAT];
+#pragma unroll
+            for (int t = 0; t < PAT; ++t) pat[t] = chunk_at<S::kHalf>(w * 32 + t * RPI + lane / CH, lane % CH);
             // All of item x's copies of this thread have landed: clean what must
             // be, and hand it over.
             auto finish = [&](int x) {
                 const uint32_t slot = sbase + S::kRing + (x % NS) * S::kMat;
                 if ((x & 1) && job.template mixed<PREC>(sight, pos_of(x >> 1))) {
-                    bool bad = false;
-#pragma unroll 4
+                    // An exponent of all ones plus one of its lowest bit carries into the
+                    // sign's place, which the mask has cleared, and no further.
+                    uint32_t found = 0;
+#pragma unroll
                     for (int t = 0; t < NI; ++t) {
-                        const uint32_t at = slot + chunk_at<S::kHalf>(w * 32 + t * RPI + lane / CH, lane % CH);
-                        const uint4 v = lds128(at);
-                        const uint4 u = make_uint4(clean16(v.x), clean16(v.y), clean16(v.z), clean16(v.w));
-                        if (u.x != v.x || u.y != v.y || u.z != v.z || u.w != v.w) {
-                            bad = true;
-                            sts128(at, u);
+                        const uint4 v = lds128(slot + pat[t % PAT] + (t / PAT) * 1024);
+                        found |= ((v.x & 0x7C007C00u) + 0x04000400u) | ((v.y & 0x7C007C00u) + 0x04000400u) |
+                                 ((v.z & 0x7C007C00u) + 0x04000400u) | ((v.w & 0x7C007C00u) + 0x04000400u);
+                    }
+                    const bool bad = (found & 0x80008000u) != 0;
+                    if (bad) {
+#pragma unroll 1
+                        for (int t = 0; t < NI; ++t) {
+                            const uint32_t at = slot + chunk_at<S::kHalf>(w * 32 + t * RPI + lane / CH, lane % CH);
+                            const uint4 v = lds128(at);
+                            sts128(at, make_uint4(clean16(v.x), clean16(v.y), clean16(v.z), clean16(v.w)));
                         }
                     }
                     if (bad) {
@@ -483,12 +497,6 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
                 ok = __all_sync(0xffffffffu, wait(bar, parity));
                 return ok;
             };
-            // Shared offsets of this thread's copies within the warp's 32 rows: they
-            // repeat every 8 rows, up to the rows themselves.
-            constexpr int PAT = 8 / RPI;
-            uint32_t pat[PAT];
-#pragma unroll
-            for (int t = 0; t < PAT; ++t) pat[t] = chunk_at<S::kHalf>(w * 32 + t * RPI + lane / CH, lane % CH);
             for (int i = 0; i < n && ok; ++i) {
                 const uint32_t row = ahead;
                 ahead = look(i + 1);
@@ -760,7 +768,7 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
 #pragma unroll
                         for (int u = 0; u < 4; ++u)
                             far[u] = max3(far[u], fabsf(x[c + 2 * u]), fabsf(x[c + 2 * u + 1]));
-                    if (__any_sync(0xffffffffu, fmaxf(fmaxf(far[0], far[1]), fmaxf(far[2], far[3])) > (PREC ? 1.0f : 0.7f))) {
+                    if (__any_sync(0xffffffffu, fmaxf(fmaxf(far[0], far[1]), fmaxf(far[2], far[3])) > (PREC ? 1.0f : 0.5f))) {
 #pragma unroll
                         for (int c = 0; c < kRows; ++c) x[c] = tanh_far(x[c]);
                     } else {
@@ -899,7 +907,7 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
                     const int j0 = pos_of(i);
                     if (!job.template mixed<PREC>(sight, j0)) continue;
 #pragma unroll 1
-                    for (int j = j0; j < min(j0 + kRows, sight.n); ++j) {
+                    for (int j = j0; j < min(j0 + kRows, sight.limit); ++j) {
                         const uint32_t rw = sight.sees(pos, j) ? row_of(a, job.b, job.kvh, j) : kNoRow;
                         if (rw == kNoRow) continue;
 #pragma unroll

@@ -415,8 +415,8 @@ B200Q_API int b200q_rope_append_paged(const void* q, const void* k, const void* 
  * and sets device status bit 2. A row that sees nothing is written as zeros.
  * Non-finite keys or values reach only the rows that see them. max_q_len and
  * max_kv_len, upper bounds of the sequences' rows and of kv_len, choose the
- * kernel and how the keys are split; rows of a sequence past max_q_len may be
- * left unwritten. scale > 0. q and out 16-byte aligned, strides a multiple of 16 bytes. */
+ * kernel and how the keys are split; a sequence with more rows than max_q_len
+ * may be left unwritten. out may be q. scale > 0. q and out 16-byte aligned, strides a multiple of 16 bytes. */
 B200Q_API int b200q_attention_paged(const void* q, int dtype, int n_tokens, int batch, const int* cu_q,
                                     const int* kv_len, int max_q_len, int max_kv_len, int n_heads, int n_kv_heads,
                                     int head_dim, long long q_stride, void* out, long long out_stride, float scale,

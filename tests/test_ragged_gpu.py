@@ -662,3 +662,35 @@ def test_graph_with_a_split_and_changing_lengths():
         _clean()
         _check_attend(c, 0, batch, q, out)
         assert (out[sum(ql):] == 2).all()
+
+
+@pytest.mark.parametrize("lens", ["few", "prompts"])
+def test_lengths_past_the_table_and_in_place(lens):
+    """kv_len past what the page table reaches (the C entry point's caller may
+    set it so): the positions past it are hidden and recorded, however far the
+    length is off; the others give what they give. out may be q."""
+    import torch
+
+    from cybel_b200 import _native
+
+    ql, kl = LENS[lens]
+    c, batch = _cache(ql, kl, 2, 128, 48, False, seed=2, poison=True)
+    q = torch.randn(batch.n_tokens, 4, 128, device="cuda").half()
+    want = c.attend(0, q, batch)
+    buf = q.clone()
+    assert c.attend(0, buf, batch, out=buf) is buf and torch.equal(buf, want)
+    _clean()
+    reach = c.pages_per_seq * 48
+    for far in (reach + 1, 2 ** 31 - 1):
+        batch.kv_len.copy_(torch.tensor(kl, dtype=torch.int32))
+        batch.kv_len[0] = far
+        out = c.attend(0, q, batch)
+        torch.cuda.synchronize()
+        with pytest.raises(_native.NativeError):
+            _native.check_device(0)
+        # (the sequence's own rows see what the rest of its last page holds: NaN here)
+        assert torch.equal(out[ql[0]:], want[ql[0]:])
+    batch.kv_len[0] = -5
+    out = c.attend(0, q, batch)
+    _clean()
+    assert (out[:ql[0]] == 0).all() and torch.equal(out[ql[0]:], want[ql[0]:])
