@@ -19,17 +19,26 @@
 //  * warps 12, 13: issue the MMAs of tile 0, 1 (one warp for both took 4850
 //    clocks a step, issuing one tile's while the other's were due).
 //
-// fp32 rows: q and the weights are each two fp16 parts (22 bits), both
-// products run twice into the same accumulators; Q8 scales multiply scores and
+// Q8 codes enter the products as they are; their scales multiply scores and
 // weights in fp32, the latter relative to a power of two above the scales so
-// far. fp16 rows take Q8 keys and values as code x scale rounded to fp16, which
-// is what their own type carries (2^-12 of a key's element moves a score by
-// 2^-12 / sqrt(head) of its size at random, an output by less than its own
-// rounding) and spares the softmax warps two products per score, half as much
-// again as all they do otherwise.
+// far. (Code x scale rounded to fp16 for the products took 176 us instead of
+// 272 at 4096 tokens, 32/8 heads, but each of the two roundings was as large as
+// the output's own, and the error against 64 bits 2.4 times as large instead of
+// 1.4 times. The weights' rounding to fp16 makes the rest of that factor.)
+//
+// fp32 rows: q and the weights are each two fp16 parts (22 bits), and both
+// products run twice into the same accumulators, the low parts first. The
+// tensor cores cut a sum off at each 16 products: over thousands of positions
+// that shrank outputs by 0.035 x 2^-24 per position and spread them half as
+// much. So a product covers 64 positions and 64 columns of the head in an
+// accumulator of its own beside the weights, and the softmax warps add it to
+// the output, which costs 370 us instead of 267 at 4096 tokens and makes the
+// error 4e-7 instead of 2e-5 at 8000 positions. (fp16 rows keep the plain sum:
+// its error reaches that of their own rounding beyond 100 000 positions a CTA.)
 // The output is rescaled in tensor memory by the softmax warps themselves and
-// only when a row's maximum rose by 2^kRise since the last time: the product
-// before is complete by then, because the barrier of S covers it. The weights
+// only when a row's maximum rose by 2^kRise since the last time (fp32 rows: with
+// the next addition): the product before is complete by then, because the
+// barrier of S covers it. The weights
 // are handed over in two halves, so that the product starts under the second
 // half's exponentials.
 //
@@ -114,7 +123,7 @@ struct Tile {
     static constexpr int kParts = PREC ? 2 : 1;
     static constexpr int kQ = kTiles * kParts * kMat;
     static constexpr int kMeta = PREC ? 2 : 4;              // steps of per-position data in flight
-    static constexpr int kMetaBytes = kMeta * static_cast<int>(sizeof(Meta<PREC && Q8>));
+    static constexpr int kMetaBytes = kMeta * static_cast<int>(sizeof(Meta<Q8>));
     static constexpr int kBarBytes = 320;
     static constexpr int kRest = kMetaBytes + kBarBytes + kBadWords * 4 + 128;
     static constexpr int kFree = (227 * 1024 - kQ - kRest) / kMat;
@@ -223,7 +232,7 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
     using T = typename std::conditional<PREC, float, __half>::type;
     constexpr int NS = S::NS;
     constexpr int kMeta = S::kMeta;
-    constexpr bool SC = PREC && Q8;  // scales beside the codes; fp16 rows get them multiplied in
+    constexpr bool SC = Q8;  // scales beside the codes
     extern __shared__ __align__(1024) uint8_t smem[];
     Job* job_s = reinterpret_cast<Job*>(smem + S::kJob);
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + S::kJob + 120);
@@ -240,6 +249,8 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
     auto mempty = [&](int i) { return bar0 + 8u * (2 * NS + kMeta + i % kMeta); };
     auto qfull = [&](int t) { return bar0 + 8u * (2 * NS + 2 * kMeta + t); };
     auto sready = [&](int t) { return bar0 + 8u * (2 * NS + 2 * kMeta + kTiles + t); };
+    // fp16 rows: half of the weights is in place. fp32 rows: the softmax warps are
+    // through with what the next product overwrites (0), a product is complete (1).
     auto pready = [&](int t, int half) { return bar0 + 8u * (2 * NS + 2 * kMeta + 2 * kTiles + 2 * t + half); };
     const uint32_t done = bar0 + 8u * (2 * NS + 2 * kMeta + 4 * kTiles);
     auto turn = [&](int t, int w) { return done + 8u * (1 + 4 * t + w); };
@@ -256,7 +267,7 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
             mbar_init(qfull(t), kRows);
             mbar_init(sready(t), 1);
             mbar_init(pready(t, 0), 4);
-            mbar_init(pready(t, 1), 4);
+            mbar_init(pready(t, 1), PREC ? 1 : 4);
             for (int w = 0; w < 4; ++w) mbar_init(turn(t, w), 1);
         }
         mbar_init(done, kTiles);
@@ -353,7 +364,7 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(issuer_regs(Q8)));
         if (warp < 12 + kTiles) {
             // ---------------- MMA issuer of tile t ----------------
-            constexpr uint32_t idS = idesc_of(kRows, false), idO = idesc_of(D, true);
+            constexpr uint32_t idS = idesc_of(kRows, false), idO = idesc_of(PREC ? 64 : D, true);
             const int t = warp - 12;
             const Steps steps(sight, list, i0, job.lo[t], job.hi[t]);
             const uint32_t ts = tmem + t * kRows, to = tmem + kO + t * D;
@@ -365,6 +376,7 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
             if (elect_one()) {
                 bool ok = wait(qfull(t), 0);
                 int np = 0;  // steps so far
+                int go = 0;  // PREC: products that waited for the softmax warps
                 for (int s = 0; s <= n && ok; ++s) {
                     const int ki = 2 * s, vi = 2 * s - 1;
                     const bool pv = s > 0 && steps.has(s - 1), qk = s < n && steps.has(s);
@@ -373,28 +385,42 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
                         const uint64_t v = v0 + ((vi % NS) * (S::kMat >> 4));
 #pragma unroll
                         for (int half = 0; half < 2; ++half) {
-                            ok = ok && wait(pready(t, half), (np - 1) & 1);
-                            if (!ok) break;
-                            tc_fence_after();
+                            if constexpr (PREC) {
 #pragma unroll
-                            for (int part = 0; part < S::kParts; ++part)
+                                for (int d = 0; d < D / 64; ++d) {
+                                    ok = ok && wait(pready(t, 0), go++ & 1);
+                                    if (!ok) break;
+                                    tc_fence_after();
+#pragma unroll
+                                    for (int k = 0; k < 8; ++k)  // low parts first
+                                        tc_mma_f16_ts(ts + 64, ts + (k < 4 ? 32 + k * 8 : (k - 4) * 8),
+                                                      v + d * (S::kHalf >> 4) + (4 * half + (k & 3)) * (2048 >> 4), idO,
+                                                      k > 0 ? 1u : 0u);
+                                    tc_commit(pready(t, 1));
+                                }
+                            } else {
+                                ok = ok && wait(pready(t, half), (np - 1) & 1);
+                                if (!ok) break;
+                                tc_fence_after();
 #pragma unroll
                                 for (int k = 4 * half; k < 4 * half + 4; ++k)
-                                    tc_mma_f16_ts(to, ts + part * 64 + k * 8, v + k * (2048 >> 4), idO,
-                                                  np > 1 || part > 0 || k > 0 ? 1u : 0u);
+                                    tc_mma_f16_ts(to, ts + k * 8, v + k * (2048 >> 4), idO, np > 1 || k > 0 ? 1u : 0u);
+                            }
                         }
                     }
                     if (!ok) break;
                     if (qk) {
+                        if (PREC && np > 0) ok = wait(pready(t, 0), go++ & 1);
+                        if (!ok) break;
                         tc_fence_after();
                         const uint64_t kk = k0 + ((ki % NS) * (S::kMat >> 4));
 #pragma unroll
-                        for (int part = 0; part < S::kParts; ++part)
+                        for (int part = S::kParts - 1; part >= 0; --part)  // low parts first
 #pragma unroll
                             for (int k = 0; k < D / 16; ++k) {
                                 const uint32_t off = ((k >> 2) * S::kHalf + (k & 3) * 32) >> 4;
                                 tc_mma_f16(ts, q0 + ((part * S::kMat) >> 4) + off, kk + off, idS,
-                                           part > 0 || k > 0 ? 1u : 0u);
+                                           part < S::kParts - 1 || k > 0 ? 1u : 0u);
                             }
                         tc_commit(sready(t));
                         ++np;
@@ -548,7 +574,7 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
                                        lane % CH);
                 }
             };
-            auto put = [&](const uint4 (&reg)[NI], int x, uint32_t scale) {
+            auto put = [&](const uint4 (&reg)[NI], int x) {
                 const uint32_t slot = sbase + S::kRing + (x % NS) * S::kMat;
 #pragma unroll
                 for (int t = 0; t < NI; ++t) {
@@ -558,32 +584,12 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
                     uint32_t h[8];
 #pragma unroll
                     for (int k = 0; k < 8; ++k) h[k] = codes_fp16(u[k >> 1], (k & 1) ? 0x4342 : 0x4140);
-                    if constexpr (!PREC) {
-                        // code x scale rounded once to fp16: the scale as two parts
-                        const uint32_t sc = __shfl_sync(0xffffffffu, scale, t * RPI + lane / CH);
-                        const __half2 s2 = *reinterpret_cast<const __half2*>(&sc);
-                        const __half2 hi = __low2half2(s2), lo = __high2half2(s2);
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            const __half2 cd = *reinterpret_cast<const __half2*>(&h[k]);
-                            const __half2 v = __hfma2(cd, hi, __hmul2(cd, lo));
-                            h[k] = *reinterpret_cast<const uint32_t*>(&v);
-                        }
-                    }
                     sts128(slot + chunk_at<S::kHalf>(row, c), make_uint4(h[0], h[1], h[2], h[3]));
                     sts128(slot + chunk_at<S::kHalf>(row, c + 1), make_uint4(h[4], h[5], h[6], h[7]));
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(kvfull(x));
-            };
-            // A scale as fp16 parts hi | lo, 22 bits of it (the low part of one that is
-            // not finite would be NaN: it is left out).
-            auto split = [](float sc) {
-                const __half hi = __float2half_rn(sc);
-                const float rest = sc - __half2float(hi);
-                const __half lo = __float2half_rn(fabsf(rest) < INFINITY ? rest : 0.0f);
-                return static_cast<uint32_t>(__half_as_ushort(hi)) | (static_cast<uint32_t>(__half_as_ushort(lo)) << 16);
             };
             uint32_t row = ahead;
             ahead = look(1);
@@ -596,17 +602,16 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
                 ok = __all_sync(0xffffffffu, wait(mempty(i), ((i / kMeta) & 1) ^ 1));
                 if (!ok) break;
                 put_meta(i, row);
-                const uint32_t ks2 = split(ks_next), vs2 = split(vs_next);
                 row = ahead;
                 scales_of(row);
                 ahead = look(i + 2);
                 ok = __all_sync(0xffffffffu, wait(kvempty(2 * i), ((2 * i / NS) & 1) ^ 1));
                 if (!ok) break;
-                put(kreg, 2 * i, ks2);
+                put(kreg, 2 * i);
                 fetch(kreg, a.kv.k, row);
                 ok = __all_sync(0xffffffffu, wait(kvempty(2 * i + 1), (((2 * i + 1) / NS) & 1) ^ 1));
                 if (!ok) break;
-                put(vreg, 2 * i + 1, vs2);
+                put(vreg, 2 * i + 1);
                 fetch(vreg, a.kv.v, row);
             }
         }
@@ -692,6 +697,7 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
         float m = -INFINITY, l = 0.0f;
         float E = 0.0f, log_E = 0.0f;  // SC: weights, their sum and the output are relative to E
         int steps = 0;
+        int drained = 0;  // PREC: products taken over so far
         bool ok = true;
         for (int i = 0; i < n && ok; ++i) {
             ok = __all_sync(0xffffffffu, wait(mfull(i), (i / kMeta) & 1));
@@ -800,6 +806,7 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
                     if (!(see[c >> 5] & (1u << (c & 31)))) x[c] = -INFINITY;
             }
             // ---- the reference maximum
+            float keep = 1.0f;  // PREC: what the output so far is worth from now on
             {
                 float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -813,7 +820,8 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
                     const float f = (m == -INFINITY ? 1.0f : ex2(m - mn)) * (steps > 0 ? unit : 1.0f);
                     m = mn;
                     l *= f;
-                    if (steps > 0) {
+                    keep = f;
+                    if (!PREC && steps > 0) {
 #pragma unroll
                         for (int c = 0; c < D; c += 16) {
                             float o[16];
@@ -832,6 +840,7 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
             // ---- weights, a quarter of the positions at a time
             const float base = m == -INFINITY ? 0.0f : kLift - m - log_E + row_off;
             float2 s2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+            uint32_t parts[PREC ? 4 : 1][16];  // PREC: the second half's, kept until the first half's products are done
 #pragma unroll
             for (int quarter = 0; quarter < 4; ++quarter) {
                 if (quarter == 3 && lane == 0) mbar_arrive(next_turn);  // its first loads run under this one's tail
@@ -859,17 +868,64 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
                     __syncwarp();
                     if (lane == 0) mbar_arrive(pready(t, 0));
                 }
-                tmem_st16(ts + quarter * 16, hi16);
-                if constexpr (PREC) tmem_st16(ts + 64 + quarter * 16, lo16);
+                if constexpr (!PREC) {
+                    tmem_st16(ts + quarter * 16, hi16);
+                } else if (quarter < 2) {
+                    tmem_st16(ts + quarter * 16, hi16);
+                    tmem_st16(ts + 32 + quarter * 16, lo16);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) parts[quarter - 2][k] = hi16[k], parts[quarter][k] = lo16[k];
+                }
             }
             const float2 st = add2(s2[0], s2[1]);
             l += st.x + st.y;
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(pready(t, 1));
-                mbar_arrive(mempty(i));
+            if constexpr (PREC) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(mempty(i));
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                    for (int d = 0; d < D / 64; ++d) {
+                        ok = __all_sync(0xffffffffu, wait(pready(t, 1), drained++ & 1));
+                        if (!ok) break;
+                        tc_fence_after();
+                        const bool add = half > 0 || steps > 0;
+                        const float f = half > 0 ? 1.0f : keep;
+#pragma unroll
+                        for (int c = 0; c < 64; c += 16) {
+                            float o[16], y[16];
+                            tmem_ld16(ts + 64 + c, y);
+                            if (add) tmem_ld16(to + 64 * d + c, o);
+                            tmem_wait_ld();
+                            tmem_loaded16(y);
+                            if (add) {
+                                tmem_loaded16(o);
+#pragma unroll
+                                for (int k = 0; k < 16; k += 2)
+                                    put2(y + k, fma2(make_float2(o[k], o[k + 1]), both(f), make_float2(y[k], y[k + 1])));
+                            }
+                            tmem_st16(to + 64 * d + c, y);
+                        }
+                        if (half == 0 && d == D / 64 - 1) {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) tmem_st16(ts + k * 16, parts[k]);
+                        }
+                        tmem_wait_st();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(pready(t, 0));
+                    }
+                }
+                if (!ok) break;
+            } else {
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(pready(t, 1));
+                    mbar_arrive(mempty(i));
+                }
             }
             ++steps;
         }
