@@ -22,7 +22,7 @@
 // Q8 codes enter the products as they are; their scales multiply scores and
 // weights in fp32, the latter relative to a power of two above the scales so
 // far. (Code x scale rounded to fp16 for the products took 176 us instead of
-// 272 at 4096 tokens, 32/8 heads, but each of the two roundings was as large as
+// 208 at 4096 tokens, 32/8 heads, but each of the two roundings was as large as
 // the output's own, and the error against 64 bits 2.4 times as large instead of
 // 1.4 times. The weights' rounding to fp16 makes the rest of that factor.)
 //
@@ -443,6 +443,10 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
             return (j <= hi_seen && (j < sight.pre || j >= lo_seen)) ? row_of(a, job.b, job.kvh, j) : kNoRow;
         };
         float ks_next = 0.0f, vs_next = 0.0f;  // Q8: the scales of the row looked up last
+        // fp16 rows of one factor: it is part of the keys' scales where the scores are
+        // shaped before the exponential.
+        const float ks_mult = PREC || (a.cap == 0.0f && !a.slopes) ? 1.0f
+                              : a.scale * (a.cap > 0.0f ? 1.0f / a.cap : kLog2e);
         auto scales_of = [&](uint32_t row) {
             if constexpr (Q8) {
                 ks_next = row != kNoRow ? __ldg(a.kv.ks + row) : 0.0f;
@@ -461,7 +465,7 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
                 }
             }
             if constexpr (SC) {
-                m.ks[r] = ks_next;
+                m.ks[r] = ks_next * ks_mult;
                 m.vs[r] = vs_next;
                 const float mx = fabsf(vs_next) < INFINITY ? fabsf(vs_next) : 0.0f;
                 const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(mx));
@@ -759,14 +763,16 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
 #pragma unroll
                 for (int c = 0; c < kRows; c += 4) {
                     const float4 k = lds_f4(ks_at + c * 4);
-                    put2(x + c, mul2(make_float2(x[c], x[c + 1]), make_float2(k.x, k.y)));
-                    put2(x + c + 2, mul2(make_float2(x[c + 2], x[c + 3]), make_float2(k.z, k.w)));
+                    // (multiplied as pairs, 120 registers of x were spilled: 272 us)
+                    x[c] *= k.x, x[c + 1] *= k.y, x[c + 2] *= k.z, x[c + 3] *= k.w;
                 }
             }
             if (shaped) {
-                const float f1 = a.cap > 0.0f ? mult * inv_cap : mult * kLog2e;
+                if (PREC || !SC) {
+                    const float f1 = a.cap > 0.0f ? mult * inv_cap : mult * kLog2e;
 #pragma unroll
-                for (int c = 0; c < kRows; c += 2) put2(x + c, mul2(make_float2(x[c], x[c + 1]), both(f1)));
+                    for (int c = 0; c < kRows; c += 2) put2(x + c, mul2(make_float2(x[c], x[c + 1]), both(f1)));
+                }
                 if (a.cap > 0.0f) {
                     float far[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
