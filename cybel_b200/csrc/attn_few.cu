@@ -7,12 +7,17 @@
 // time, each as two fp16 parts hi + lo of its value (22 bits, after scaling
 // the row by a power of two) in rows r and r + 8, so that one product gives
 // both and their sum stays in a lane. The softmax weights of fp32 rows are
-// split in the same way before the second product.
+// split in the same way before the second product. So are those of fp16 rows
+// where no sequence has more than 8 of them (a decode step): the upper half of
+// the product would stay empty, and a lane has one row's exponentials instead
+// of two: 64 rows of 64/8 heads over 100-8000 Q8 positions 135 -> 125 us, one
+// row of 32/8 heads over 2048 9.5 -> 8.6, and the error against 64 bits 1.0
+// times the plain form's instead of 1.4 times.
 //
-// A warp takes every (4 C)-th tile of 16 positions through a cp.async ring of
+// A warp takes every (4 C)-th tile of 16 or 32 positions through a cp.async ring of
 // its own and keeps a running maximum, sum and output: the warps share
 // nothing until the end, so no barrier stands between the loads. The CTAs of
-// a cluster (C, up to 8) share one block of rows; their partial outputs are
+// a cluster (C, up to 16) share one block of rows; their partial outputs are
 // joined in shared memory over the cluster, in a fixed order, without a
 // workspace, a counter or a second launch. The page of the next tile to load
 // is looked up one tile ahead of its loads.
@@ -37,9 +42,9 @@ constexpr int kMaxCluster = 16;  // beyond 8 only where the device allows it
 constexpr float kRise = 4.0f;    // a row's reference maximum follows once exceeded by this (log2)
 constexpr float kLift = 10.0f;   // weights are 2^(score - maximum + kLift): at most 2^14 in fp16
 
-template <int D, bool PREC, bool Q8>
+template <int D, bool SPLIT, bool Q8>
 struct Few {
-    static constexpr int R = PREC ? 8 : 16;               // rows per block
+    static constexpr int R = SPLIT ? 8 : 16;               // rows per block
     static constexpr int RB = Q8 ? D : 2 * D;             // bytes per stored row
     static constexpr int CH = RB / 16;                    // 16-byte chunks per row
     // Positions per tile: more of them give a warp more independent products;
@@ -117,15 +122,16 @@ __device__ __forceinline__ int v_chunk(int r, int c) {
     return D == 128 ? c ^ (r & 6) : c ^ ((r >> 1) & 3);
 }
 
-template <int D, bool PREC, bool Q8>
+template <int D, bool FP32, bool SPLIT, bool Q8>
 __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) b200q_attn_few_kernel(const AttnArgs a) {
-    using F = Few<D, PREC, Q8>;
-    using T = typename std::conditional<PREC, float, __half>::type;
+    using F = Few<D, SPLIT, Q8>;
+    using T = typename std::conditional<FP32, float, __half>::type;
+    static_assert(SPLIT || !FP32, "fp32 rows have two parts");
     constexpr int R = F::R, KS = D / 16, NB = D / 8, NS = F::NS, kTile = F::kTile;
     constexpr int NK = kTile / 8;  // blocks of 8 positions
     constexpr uint32_t kAll = kTile == 32 ? 0xFFFFFFFFu : 0xFFFFu;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ uint32_t present[kWarps][8];  // per stage: which of its 16 positions have a row
+    __shared__ uint32_t present[kWarps][8];  // per stage: which of its positions have a row
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     float2* ml = reinterpret_cast<float2*>(smem + kWarps * F::kWarpBytes);  // [kWarps][R] max, sum
     float2* ml_cta = ml + kWarps * R;                                       // [R]
@@ -147,8 +153,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) b200q_attn_few_kernel
     const int p0 = s.n - (rr.y - rr.x);
     const int p_lo = p0 + r0 / a.group, p_hi = p0 + (r0 + nr - 1) / a.group;
 
-    // This lane's rows: g, and for fp16 g + 8.
-    constexpr int NR = PREC ? 1 : 2;
+    // This lane's rows: g, and without low parts g + 8.
+    constexpr int NR = SPLIT ? 1 : 2;
     int pos[NR];
     float slope[NR], mult[NR];
     uint32_t qa[KS][4];
@@ -170,7 +176,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) b200q_attn_few_kernel
         for (int ks = 0; ks < KS; ++ks) {
             const int e0 = Q8 ? (ks >> 2) * 64 + c * 16 + (ks & 3) * 4 : ks * 16 + 2 * c;
             const int e1 = Q8 ? e0 + 2 : e0 + 8;
-            if constexpr (PREC) {
+            if constexpr (FP32) {
                 const float2 x = have ? *reinterpret_cast<const float2*>(q + e0) : make_float2(0.0f, 0.0f);
                 const float2 y = have ? *reinterpret_cast<const float2*>(q + e1) : make_float2(0.0f, 0.0f);
                 v[ks][0] = x.x, v[ks][1] = x.y, v[ks][2] = y.x, v[ks][3] = y.y;
@@ -179,10 +185,11 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) b200q_attn_few_kernel
             } else {
                 qa[ks][i] = have ? *reinterpret_cast<const uint32_t*>(q + e0) : 0u;
                 qa[ks][2 + i] = have ? *reinterpret_cast<const uint32_t*>(q + e1) : 0u;
+                if constexpr (SPLIT) qa[ks][1] = qa[ks][3] = 0u;  // fp16 as it is
             }
         }
         mult[i] = a.scale;
-        if constexpr (PREC) {
+        if constexpr (FP32) {
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
             // |q| / E below 1: parts of q 2^10 / E, the smallest of them 2^-34 of the largest element
@@ -326,12 +333,13 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) b200q_attn_few_kernel
                 const float2 k2 = lds_f2(st + 2 * kTile * F::RB + (nb * 8 + 2 * c) * 4);
                 ks0 = k2.x, ks1 = k2.y;
             }
-            if constexpr (PREC) {
+            if constexpr (FP32) {
                 x[0][2 * nb] = (sc[nb][0] + sc[nb][2]) * ks0;
                 x[0][2 * nb + 1] = (sc[nb][1] + sc[nb][3]) * ks1;
             } else {
                 x[0][2 * nb] = sc[nb][0] * ks0, x[0][2 * nb + 1] = sc[nb][1] * ks1;
-                x[NR - 1][2 * nb] = sc[nb][2] * ks0, x[NR - 1][2 * nb + 1] = sc[nb][3] * ks1;
+                if constexpr (!SPLIT)
+                    x[NR - 1][2 * nb] = sc[nb][2] * ks0, x[NR - 1][2 * nb + 1] = sc[nb][3] * ks1;
             }
         }
         const bool whole = bits == kAll && s.all(p_lo, p_hi, j0, j0 + kTile - 1);
@@ -401,7 +409,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) b200q_attn_few_kernel
                 l[i2] *= f;
 #pragma unroll
                 for (int n = 0; n < NB; ++n) {
-                    if constexpr (PREC) {
+                    if constexpr (SPLIT) {
 #pragma unroll
                         for (int v = 0; v < 4; ++v) o[n][v] *= f * unit;
                     } else {
@@ -425,7 +433,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) b200q_attn_few_kernel
                     l[i2] += p[v];
                     if constexpr (Q8) p[v] = x[i2][4 * f + v] == -INFINITY ? 0.0f : p[v] * vs[4 * f + v];
                 }
-                if constexpr (PREC) {
+                if constexpr (SPLIT) {
                     pa[f][0] = pack2(p[0], p[1]);
                     pa[f][2] = pack2(p[2], p[3]);
                     const float2 h0 = unpack2(pa[f][0]), h1 = unpack2(pa[f][2]);
@@ -539,7 +547,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) b200q_attn_few_kernel
                 const int col = 2 * c + v;
                 const int e = Q8 ? col * NB + n : n * 8 + col;
                 // (the low parts of weights turn an infinite value into NaN: leave them out then)
-                const float val = !PREC ? o[n][2 * i + v]
+                const float val = !SPLIT ? o[n][2 * i + v]
                                         : o[n][v] + (fabsf(o[n][2 + v]) < INFINITY ? o[n][2 + v] : 0.0f);
                 part[(g + 8 * i) * D + e] = val * out_unit;
             }
@@ -607,9 +615,9 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) b200q_attn_few_kernel
     cluster_sync();  // no CTA leaves while another reads its shared memory
 }
 
-template <int D, bool PREC, bool Q8>
+template <int D, bool FP32, bool SPLIT, bool Q8>
 int launch_few(const AttnArgs& a0, int max_rows, int max_kv, int sms, cudaStream_t st) {
-    using F = Few<D, PREC, Q8>;
+    using F = Few<D, SPLIT, Q8>;
     static_assert(F::kTotal <= 226 * 1024 / kCtasPerSm - 1024, "resident CTAs");
     AttnArgs a = a0;
     a.row_blocks = (max_rows + F::R - 1) / F::R;
@@ -621,9 +629,9 @@ int launch_few(const AttnArgs& a0, int max_rows, int max_kv, int sms, cudaStream
         std::lock_guard<std::mutex> lk(mu);
         const uint64_t bit = dev < 64 ? 1ull << dev : 0;
         if (!(done & bit)) {
-            if (cudaFuncSetAttribute(b200q_attn_few_kernel<D, PREC, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+            if (cudaFuncSetAttribute(b200q_attn_few_kernel<D, FP32, SPLIT, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      F::kTotal) != cudaSuccess ||
-                cudaFuncSetAttribute(b200q_attn_few_kernel<D, PREC, Q8>, cudaFuncAttributeNonPortableClusterSizeAllowed,
+                cudaFuncSetAttribute(b200q_attn_few_kernel<D, FP32, SPLIT, Q8>, cudaFuncAttributeNonPortableClusterSizeAllowed,
                                      1) != cudaSuccess)
                 return B200Q_ECUDA;
             done |= bit;
@@ -655,12 +663,12 @@ int launch_few(const AttnArgs& a0, int max_rows, int max_kv, int sms, cudaStream
         attr[1].val.programmaticStreamSerializationAllowed = 1;
         cfg.numAttrs = 2;
     }
-    cudaError_t e = cudaLaunchKernelEx(&cfg, b200q_attn_few_kernel<D, PREC, Q8>, a);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, b200q_attn_few_kernel<D, FP32, SPLIT, Q8>, a);
     if (e != cudaSuccess && c > 8) {  // no room for clusters of 16 (a partitioned device): the portable size
         cudaGetLastError();
         attr[0].val.clusterDim.x = 8;
         cfg.gridDim.x = static_cast<unsigned>(units * 8);
-        e = cudaLaunchKernelEx(&cfg, b200q_attn_few_kernel<D, PREC, Q8>, a);
+        e = cudaLaunchKernelEx(&cfg, b200q_attn_few_kernel<D, FP32, SPLIT, Q8>, a);
     }
     return e == cudaSuccess ? B200Q_OK : B200Q_ECUDA;
 }
@@ -668,11 +676,13 @@ int launch_few(const AttnArgs& a0, int max_rows, int max_kv, int sms, cudaStream
 }  // namespace
 
 int launch_attn_few(const AttnArgs& a, int hd, bool fp32, bool q8, int max_rows, int max_kv, int sms, cudaStream_t st) {
-#define B200Q_FEW(D)                                                                                       \
-    (fp32 ? (q8 ? launch_few<D, true, true>(a, max_rows, max_kv, sms, st) : launch_few<D, true, false>(a, max_rows, max_kv, sms, st)) \
-          : (q8 ? launch_few<D, false, true>(a, max_rows, max_kv, sms, st) : launch_few<D, false, false>(a, max_rows, max_kv, sms, st)))
+#define B200Q_FEW3(D, FP32, SPLIT)                                             \
+    (q8 ? launch_few<D, FP32, SPLIT, true>(a, max_rows, max_kv, sms, st) \
+        : launch_few<D, FP32, SPLIT, false>(a, max_rows, max_kv, sms, st))
+#define B200Q_FEW(D) (fp32 ? B200Q_FEW3(D, true, true) : max_rows <= 8 ? B200Q_FEW3(D, false, true) : B200Q_FEW3(D, false, false))
     return hd == 128 ? B200Q_FEW(128) : B200Q_FEW(64);
 #undef B200Q_FEW
+#undef B200Q_FEW3
 }
 
 }  // namespace b200q
