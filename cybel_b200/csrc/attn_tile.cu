@@ -30,11 +30,12 @@
 // products run twice into the same accumulators, the low parts first. The
 // tensor cores cut a sum off at each 16 products: over thousands of positions
 // that shrank outputs by 0.035 x 2^-24 per position and spread them half as
-// much. So a product covers 64 positions and 64 columns of the head in an
-// accumulator of its own beside the weights, and the softmax warps add it to
-// the output, which costs 370 us instead of 267 at 4096 tokens and makes the
+// much. So a product covers a step (head 64) or 64 positions and 64 columns of
+// the head (head 128) in an accumulator of its own, and the softmax warps add it
+// to the output, which costs 370 us instead of 267 at 4096 tokens and makes the
 // error 4e-7 instead of 2e-5 at 8000 positions. (fp16 rows keep the plain sum:
 // its error reaches that of their own rounding beyond 100 000 positions a CTA.)
+//
 // The output is rescaled in tensor memory by the softmax warps themselves and
 // only when a row's maximum rose by 2^kRise since the last time (fp32 rows: with
 // the next addition): the product before is complete by then, because the
@@ -233,6 +234,10 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
     constexpr int NS = S::NS;
     constexpr int kMeta = S::kMeta;
     constexpr bool SC = Q8;  // scales beside the codes
+    // Where fp32 rows' products have accumulators of their own: of a whole step
+    // (head 64: tensor memory has room), or of 64 positions and columns at a time
+    // over the weights' place, which the next product has to wait for.
+    constexpr bool kWide = PREC && D == 64, kNarrow = PREC && D == 128;
     extern __shared__ __align__(1024) uint8_t smem[];
     Job* job_s = reinterpret_cast<Job*>(smem + S::kJob);
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + S::kJob + 120);
@@ -249,8 +254,8 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
     auto mempty = [&](int i) { return bar0 + 8u * (2 * NS + kMeta + i % kMeta); };
     auto qfull = [&](int t) { return bar0 + 8u * (2 * NS + 2 * kMeta + t); };
     auto sready = [&](int t) { return bar0 + 8u * (2 * NS + 2 * kMeta + kTiles + t); };
-    // fp16 rows: half of the weights is in place. fp32 rows: the softmax warps are
-    // through with what the next product overwrites (0), a product is complete (1).
+    // Half of the weights is in place. kNarrow: the softmax warps are through with
+    // what the next product overwrites (0), a product is complete (1).
     auto pready = [&](int t, int half) { return bar0 + 8u * (2 * NS + 2 * kMeta + 2 * kTiles + 2 * t + half); };
     const uint32_t done = bar0 + 8u * (2 * NS + 2 * kMeta + 4 * kTiles);
     auto turn = [&](int t, int w) { return done + 8u * (1 + 4 * t + w); };
@@ -267,7 +272,7 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
             mbar_init(qfull(t), kRows);
             mbar_init(sready(t), 1);
             mbar_init(pready(t, 0), 4);
-            mbar_init(pready(t, 1), PREC ? 1 : 4);
+            mbar_init(pready(t, 1), kNarrow ? 1 : 4);
             for (int w = 0; w < 4; ++w) mbar_init(turn(t, w), 1);
         }
         mbar_init(done, kTiles);
@@ -358,13 +363,15 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
     uint32_t* bad_bits = reinterpret_cast<uint32_t*>(smem + S::kBad);
     auto pos_of = [&](int i) { return list.at(i0 + i); };
     float2* ml = reinterpret_cast<float2*>(smem + S::kMl);
-    constexpr uint32_t kO = 256;  // tensor-memory columns: S (then P) of the tiles, then their outputs
+    // tensor-memory columns: S (then P) of the tiles, then their outputs, then kWide's accumulators
+    constexpr uint32_t kO = 256, kF = 384;
 
     if (warp >= 12) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(issuer_regs(Q8)));
         if (warp < 12 + kTiles) {
             // ---------------- MMA issuer of tile t ----------------
             constexpr uint32_t idS = idesc_of(kRows, false), idO = idesc_of(PREC ? 64 : D, true);
+            constexpr int kLast = S::kParts - 1;
             const int t = warp - 12;
             const Steps steps(sight, list, i0, job.lo[t], job.hi[t]);
             const uint32_t ts = tmem + t * kRows, to = tmem + kO + t * D;
@@ -376,7 +383,7 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
             if (elect_one()) {
                 bool ok = wait(qfull(t), 0);
                 int np = 0;  // steps so far
-                int go = 0;  // PREC: products that waited for the softmax warps
+                int go = 0;  // kNarrow: products that waited for the softmax warps
                 for (int s = 0; s <= n && ok; ++s) {
                     const int ki = 2 * s, vi = 2 * s - 1;
                     const bool pv = s > 0 && steps.has(s - 1), qk = s < n && steps.has(s);
@@ -385,7 +392,7 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
                         const uint64_t v = v0 + ((vi % NS) * (S::kMat >> 4));
 #pragma unroll
                         for (int half = 0; half < 2; ++half) {
-                            if constexpr (PREC) {
+                            if constexpr (kNarrow) {
 #pragma unroll
                                 for (int d = 0; d < D / 64; ++d) {
                                     ok = ok && wait(pready(t, 0), go++ & 1);
@@ -403,24 +410,28 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
                                 if (!ok) break;
                                 tc_fence_after();
 #pragma unroll
-                                for (int k = 4 * half; k < 4 * half + 4; ++k)
-                                    tc_mma_f16_ts(to, ts + k * 8, v + k * (2048 >> 4), idO, np > 1 || k > 0 ? 1u : 0u);
+                                for (int part = kLast; part >= 0; --part)  // low parts first
+#pragma unroll
+                                    for (int k = 4 * half; k < 4 * half + 4; ++k)
+                                        tc_mma_f16_ts(kWide ? tmem + kF + t * 64 : to, ts + part * 64 + k * 8,
+                                                      v + k * (2048 >> 4), idO,
+                                                      (!kWide && np > 1) || part < kLast || k > 0 ? 1u : 0u);
                             }
                         }
                     }
                     if (!ok) break;
                     if (qk) {
-                        if (PREC && np > 0) ok = wait(pready(t, 0), go++ & 1);
+                        if (kNarrow && np > 0) ok = wait(pready(t, 0), go++ & 1);
                         if (!ok) break;
                         tc_fence_after();
                         const uint64_t kk = k0 + ((ki % NS) * (S::kMat >> 4));
 #pragma unroll
-                        for (int part = S::kParts - 1; part >= 0; --part)  // low parts first
+                        for (int part = kLast; part >= 0; --part)  // low parts first
 #pragma unroll
                             for (int k = 0; k < D / 16; ++k) {
                                 const uint32_t off = ((k >> 2) * S::kHalf + (k & 3) * 32) >> 4;
                                 tc_mma_f16(ts, q0 + ((part * S::kMat) >> 4) + off, kk + off, idS,
-                                           part < S::kParts - 1 || k > 0 ? 1u : 0u);
+                                           part < kLast || k > 0 ? 1u : 0u);
                             }
                         tc_commit(sready(t));
                         ++np;
@@ -700,8 +711,27 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
         const int t_lo = job.lo[t], t_hi = job.hi[t];
         float m = -INFINITY, l = 0.0f;
         float E = 0.0f, log_E = 0.0f;  // SC: weights, their sum and the output are relative to E
+        // PREC: 64 columns of the output, o keep + the product at f (o 0 before `add`).
+        auto take = [&](uint32_t f, uint32_t o_at, bool add, float keep) {
+#pragma unroll
+            for (int c = 0; c < 64; c += 16) {
+                float o[16], y[16];
+                tmem_ld16(f + c, y);
+                if (add) tmem_ld16(o_at + c, o);
+                tmem_wait_ld();
+                tmem_loaded16(y);
+                if (add) {
+                    tmem_loaded16(o);
+#pragma unroll
+                    for (int k = 0; k < 16; k += 2)
+                        put2(y + k, fma2(make_float2(o[k], o[k + 1]), both(keep), make_float2(y[k], y[k + 1])));
+                }
+                tmem_st16(o_at + c, y);
+            }
+        };
+        float last_keep = 1.0f;  // kWide: of the step whose product is not in the output yet
         int steps = 0;
-        int drained = 0;  // PREC: products taken over so far
+        int drained = 0;  // kNarrow: products taken over so far
         bool ok = true;
         for (int i = 0; i < n && ok; ++i) {
             ok = __all_sync(0xffffffffu, wait(mfull(i), (i / kMeta) & 1));
@@ -812,7 +842,7 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
                     if (!(see[c >> 5] & (1u << (c & 31)))) x[c] = -INFINITY;
             }
             // ---- the reference maximum
-            float keep = 1.0f;  // PREC: what the output so far is worth from now on
+            float keep = 1.0f;  // PREC: what the output so far is worth from here on
             {
                 float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -841,12 +871,19 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
                     }
                 }
             }
+            if constexpr (kWide) {  // the last step's product: complete, as S is
+                if (steps > 0) {
+                    take(tmem + lanes + kF + t * 64, to, steps > 1, last_keep);
+                    tmem_wait_st();
+                }
+                last_keep = keep;
+            }
             ok = __all_sync(0xffffffffu, !wait_turn || wait(my_turn, (i - 1 + t) & 1));
             if (!ok) break;
             // ---- weights, a quarter of the positions at a time
             const float base = m == -INFINITY ? 0.0f : kLift - m - log_E + row_off;
             float2 s2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-            uint32_t parts[PREC ? 4 : 1][16];  // PREC: the second half's, kept until the first half's products are done
+            uint32_t parts[kNarrow ? 4 : 1][16];  // kNarrow: the second half's, kept until the first half's products are done
 #pragma unroll
             for (int quarter = 0; quarter < 4; ++quarter) {
                 if (quarter == 3 && lane == 0) mbar_arrive(next_turn);  // its first loads run under this one's tail
@@ -874,8 +911,9 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
                     __syncwarp();
                     if (lane == 0) mbar_arrive(pready(t, 0));
                 }
-                if constexpr (!PREC) {
+                if constexpr (!kNarrow) {
                     tmem_st16(ts + quarter * 16, hi16);
+                    if constexpr (PREC) tmem_st16(ts + 64 + quarter * 16, lo16);
                 } else if (quarter < 2) {
                     tmem_st16(ts + quarter * 16, hi16);
                     tmem_st16(ts + 32 + quarter * 16, lo16);
@@ -886,7 +924,7 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
             }
             const float2 st = add2(s2[0], s2[1]);
             l += st.x + st.y;
-            if constexpr (PREC) {
+            if constexpr (kNarrow) {
                 __syncwarp();
                 if (lane == 0) mbar_arrive(mempty(i));
 #pragma unroll
@@ -896,23 +934,7 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
                         ok = __all_sync(0xffffffffu, wait(pready(t, 1), drained++ & 1));
                         if (!ok) break;
                         tc_fence_after();
-                        const bool add = half > 0 || steps > 0;
-                        const float f = half > 0 ? 1.0f : keep;
-#pragma unroll
-                        for (int c = 0; c < 64; c += 16) {
-                            float o[16], y[16];
-                            tmem_ld16(ts + 64 + c, y);
-                            if (add) tmem_ld16(to + 64 * d + c, o);
-                            tmem_wait_ld();
-                            tmem_loaded16(y);
-                            if (add) {
-                                tmem_loaded16(o);
-#pragma unroll
-                                for (int k = 0; k < 16; k += 2)
-                                    put2(y + k, fma2(make_float2(o[k], o[k + 1]), both(f), make_float2(y[k], y[k + 1])));
-                            }
-                            tmem_st16(to + 64 * d + c, y);
-                        }
+                        take(ts + 64, to + 64 * d, half > 0 || steps > 0, half > 0 ? 1.0f : keep);
                         if (half == 0 && d == D / 64 - 1) {
 #pragma unroll
                             for (int k = 0; k < 4; ++k) tmem_st16(ts + k * 16, parts[k]);
@@ -938,6 +960,12 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
         // ---------------- output ----------------
         ok = __all_sync(0xffffffffu, wait(done, 0));
         tc_fence_after();
+        if constexpr (kWide) {
+            if (steps > 0 && ok) {
+                take(tmem + lanes + kF + t * 64, to, steps > 1, last_keep);
+                tmem_wait_st();
+            }
+        }
         const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
         const float fin = C == 1 ? inv : (SC && l > 0.0f ? E : 1.0f);
         if (C > 1) ml[t * kRows + tid] = make_float2(m, l * fin);
