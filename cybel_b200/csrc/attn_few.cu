@@ -638,14 +638,7 @@ int launch_few(const AttnArgs& a0, int max_rows, int max_kv, int sms, cudaStream
         }
     }
     const long long units = static_cast<long long>(a.r.batch) * a.kv.n_kv * a.row_blocks;
-    // CTAs per block of rows: as many as one wave holds while the blocks leave
-    // SMs idle, two where they fill more than half a wave (ragged lengths even out
-    // over the halves), and 32 positions a warp at least. Measured at 4 x 8 rows of
-    // 2000 positions: 17 us for one wave, 24 for two; 64 sequences of 100-8000: 191,
-    // 175, 186 us for 1, 2, 4.
-    const long long slots = static_cast<long long>(sms) * kCtasPerSm;
-    int c = 1;
-    while (c < kMaxCluster && (units * c * 2 <= slots || c == 1) && max_kv > c * 2 * kWarps * 32) c *= 2;
+    const int c = few_split(units, max_kv, sms);
     if (units * c > 0x7fffffffll) return B200Q_ESHAPE;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(units * c));
@@ -674,6 +667,22 @@ int launch_few(const AttnArgs& a0, int max_rows, int max_kv, int sms, cudaStream
 }
 
 }  // namespace
+
+// CTAs per block of rows: as many as one wave holds while the blocks leave SMs
+// idle, two where they fill more than half a wave (ragged lengths even out over
+// the halves), and 32 positions a warp at least. Measured at 4 x 8 rows of 2000
+// positions: 17 us for one wave, 24 for two; 64 sequences of 100-8000: 191, 175,
+// 186 us for 1, 2, 4. Clusters of 16 for three quarters of a wave only: more of
+// them do not fit the GPCs (24 of them took 36 us at 8000 positions).
+int few_split(long long units, int max_kv, int sms) {
+    const long long slots = static_cast<long long>(sms) * kCtasPerSm;
+    int c = 1;
+    while (c < kMaxCluster && (units * c * 2 <= (c * 2 < kMaxCluster ? slots : slots * 3 / 4) || c == 1) &&
+           max_kv > c * 2 * kWarps * 32)
+        c *= 2;
+    return c;
+}
+int few_slots(int sms) { return sms * kCtasPerSm; }
 
 int launch_attn_few(const AttnArgs& a, int hd, bool fp32, bool q8, int max_rows, int max_kv, int sms, cudaStream_t st) {
 #define B200Q_FEW3(D, FP32, SPLIT)                                             \

@@ -20,13 +20,26 @@ namespace {
 
 // Sequences with at most this many rows (tokens x query heads per kv head) are
 // the few-row kernel's, the others the tile kernel's. Up to 32 rows the few-row
-// kernel is as fast or faster at any batch (fp16, 8 tokens of 4 heads per kv
-// head at 2000 positions: 12 against 24 us for 1 sequence, 79 against 78 for
-// 32); at 64 rows only while its blocks of rows leave SMs idle (16 tokens: 14
-// against 25 us for 1 sequence, 32 against 28 for 4, 135 against 78 for 32).
-int few_rows(long long heads, bool fp32, int sms) {
-    const int blocks = 64 / (fp32 ? 8 : 16);
-    return heads * blocks <= sms ? 64 : 32;
+// kernel is as fast or faster at any batch (8 tokens of 4 heads per kv head at
+// 2000 positions, fp16: 12 against 19 us for 1 sequence, 80 against 79 for 32).
+// Beyond, whichever comes out ahead by what their times follow, as measured at
+// 8 kv heads, 1 to 4 sequences of 48 to 256 rows and 300 to 8000 positions: the
+// few-row kernel's the positions of a CTA and its waves, the tile kernel's the
+// steps of a CTA, however full its tiles are. (24 tokens of 4 heads per kv head
+// at 2000 positions: fp32 26 against 35 us for 2 sequences, 50 against 52 for 4;
+// fp16 14 against 19 for 1, 29 against 25 for 4. Of 360 such batches six take
+// the kernel that is slower by more than 8 percent, by 33 at most.)
+int few_rows(int batch, int n_kv, long long total_rows, int most, int max_kv, bool fp32, bool q8, int sms) {
+    if (most <= 32 || most > 256) return 32;
+    const long long fu = static_cast<long long>(batch) * n_kv * ((most + (fp32 ? 7 : 15)) / (fp32 ? 8 : 16));
+    const int fc = few_split(fu, max_kv, sms);
+    const long long fw = (fu * fc + few_slots(sms) - 1) / few_slots(sms);
+    const double few_us = 3.0 + static_cast<double>(fw) * (6.0 + (fp32 ? 0.018 : 0.021) * max_kv / fc);
+    const long long tu = tile_blocks(batch, total_rows, most, 32) * n_kv;
+    const int tc = tile_split(tu, max_kv, sms);
+    const long long steps = (max_kv + 128 * tc - 1) / (128 * tc), tw = (tu * tc + sms - 1) / sms;
+    const double step_us = fp32 ? (q8 ? 6.8 : 5.4) : (q8 ? 3.2 : 2.2);
+    return few_us < (fp32 ? 16.0 : 11.0) + step_us * static_cast<double>(steps * tw) ? 256 : 32;
 }
 
 }  // namespace
@@ -73,14 +86,17 @@ int launch_attention_paged(const void* q, int dtype, int n_tokens, int batch, co
     a.group = heads / pkv.n_kv;
     divisor(pkv.page_size, a.page_mul, a.page_shift);
     divisor(a.group, a.group_mul, a.group_shift);
-    a.few_rows = few_rows(static_cast<long long>(batch) * pkv.n_kv, dtype == B200Q_F32, dev->num_sms);
-    const bool q8 = pkv.kv_mode == B200Q_KV_Q8;
-    const long long most = static_cast<long long>(max_q_len < n_tokens ? max_q_len : n_tokens) * a.group;
-    rc = launch_attn_few(a, hd, dtype == B200Q_F32, q8, static_cast<int>(std::min<long long>(most, a.few_rows)),
-                         max_kv_len, dev->num_sms, st);
-    if (rc != B200Q_OK || most <= a.few_rows) return rc;
-    return launch_attn_tiles(a, hd, dtype == B200Q_F32, q8, static_cast<long long>(n_tokens) * a.group, max_kv_len,
-                             dev->num_sms, st);
+    const bool q8 = pkv.kv_mode == B200Q_KV_Q8, fp32 = dtype == B200Q_F32;
+    const long long total_rows = static_cast<long long>(n_tokens) * a.group;  // at most 2^30
+    const int tokens = std::min(max_q_len, n_tokens);                        // of a sequence
+    a.most_rows = tokens * a.group;
+    // Positions that a row block has to read, for the splits below.
+    const int reach = window > 0 && !prefix ? static_cast<int>(std::min<long long>(max_kv_len, static_cast<long long>(window) + tokens))
+                                            : max_kv_len;
+    a.few_rows = few_rows(batch, pkv.n_kv, total_rows, a.most_rows, reach, fp32, q8, dev->num_sms);
+    rc = launch_attn_few(a, hd, fp32, q8, std::min(a.most_rows, a.few_rows), reach, dev->num_sms, st);
+    if (rc != B200Q_OK || a.most_rows <= a.few_rows) return rc;
+    return launch_attn_tiles(a, hd, fp32, q8, total_rows, reach, dev->num_sms, st);
 }
 
 }  // namespace b200q

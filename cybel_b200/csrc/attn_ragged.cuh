@@ -22,7 +22,8 @@ struct AttnArgs {
     int page_shift;
     uint32_t group_mul;   // the same of row / group
     int group_shift;
-    int few_rows;         // sequences with at most this many rows x group are the few-row kernel's
+    int few_rows;         // sequences of at most this many rows (tokens x group) are the few-row kernel's
+    int most_rows;        // of a sequence, as the caller says
     int row_blocks;       // few-row kernel: blocks of rows per sequence and kv head
 };
 
@@ -181,5 +182,13 @@ int launch_attn_few(const AttnArgs& a, int hd, bool fp32, bool q8, int max_rows,
 
 int launch_attn_tiles(const AttnArgs& a, int hd, bool fp32, bool q8, long long total_rows, int max_kv, int sms,
                       cudaStream_t st);
+// Blocks of rows that the tile kernel is launched for, an upper bound of those
+// there are (the lengths are on the device) ...
+long long tile_blocks(int batch, long long total_rows, int most_rows, int few_rows);
+// ... and the CTAs that split the positions of each.
+int tile_split(long long units, int max_kv, int sms);
+// The few-row kernel's split of `units` blocks, and the CTAs that run at once.
+int few_split(long long units, int max_kv, int sms);
+int few_slots(int sms);
 
 }  // namespace b200q

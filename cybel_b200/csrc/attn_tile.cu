@@ -297,7 +297,8 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
             if (b >= a.r.batch) return 0;
             const int2 rr = b < 32 ? rr_lane : seq_rows(a.r, b);
             const int rows = (rr.y - rr.x) * a.group;
-            return rows > a.few_rows ? (rows + kCtaRows - 1) / kCtaRows : 0;
+            // (no more than the grid has room for, whatever the lengths say)
+            return rows > a.few_rows ? (min(rows, a.most_rows) + kCtaRows - 1) / kCtaRows : 0;
         };
         int total = 0;
         for (int b0 = 0; b0 < a.r.batch; b0 += 32) total += blocks(b0 + lane);
@@ -1100,14 +1101,9 @@ int launch_tiles(const AttnArgs& a, long long total_rows, int max_kv, int sms, c
             done |= bit;
         }
     }
-    // An upper bound of the blocks of rows: the lengths are on the device.
-    const long long seqs = std::min<long long>(a.r.batch, total_rows / (a.few_rows + 1));
-    const long long blocks = total_rows / kCtaRows + seqs;
-    if (blocks <= 0) return B200Q_OK;
-    const long long units = blocks * a.kv.n_kv;
-    // Split the positions while the blocks leave SMs idle, four steps a CTA at least.
-    int c = 1;
-    while (c < kMaxCluster && units * c * 2 <= sms && max_kv >= c * 2 * 4 * kRows) c *= 2;
+    const long long units = tile_blocks(a.r.batch, total_rows, a.most_rows, a.few_rows) * a.kv.n_kv;
+    if (units <= 0) return B200Q_OK;
+    const int c = tile_split(units, max_kv, sms);
     if (units * c > 0x7fffffffll) return B200Q_ESHAPE;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(units * c));
@@ -1129,6 +1125,22 @@ int launch_tiles(const AttnArgs& a, long long total_rows, int max_kv, int sms, c
 }
 
 }  // namespace
+
+long long tile_blocks(int batch, long long total_rows, int most_rows, int few_rows) {
+    const long long seqs = std::min<long long>(batch, total_rows / (few_rows + 1));
+    return std::min(total_rows / kCtaRows + seqs, seqs * ((most_rows + kCtaRows - 1) / kCtaRows));
+}
+
+// While the blocks leave SMs idle, two steps a CTA at least (64 tokens of 32/8
+// heads at 2000 positions, fp16: 22 us, 30 with four), and eight CTAs only for
+// four fifths of the SMs: a GPC's are not a multiple of eight (16 clusters of
+// eight took 37 us at 4000 positions, of four 26).
+int tile_split(long long units, int max_kv, int sms) {
+    int c = 1;
+    while (c < kMaxCluster && units * c * 2 <= (c * 2 < kMaxCluster ? sms : sms * 4 / 5) && max_kv >= c * 2 * 2 * kRows)
+        c *= 2;
+    return c;
+}
 
 int launch_attn_tiles(const AttnArgs& a, int hd, bool fp32, bool q8, long long total_rows, int max_kv, int sms,
                       cudaStream_t st) {

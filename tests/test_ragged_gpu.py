@@ -694,3 +694,43 @@ def test_lengths_past_the_table_and_in_place(lens):
     out = c.attend(0, q, batch)
     _clean()
     assert (out[:ql[0]] == 0).all() and torch.equal(out[ql[0]:], want[ql[0]:])
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("dtype", ["fp32", "fp16"])
+@pytest.mark.parametrize("hd,heads,kv", [(128, 8, 2), (64, 6, 2)])
+@pytest.mark.parametrize("ql,kl", [([64], [64]), ([9], [4100]), ([40, 1], [300, 2000]), ([30, 21, 64, 2], [30, 90, 70, 300]),
+                                   ([64] * 24, [64 + 20 * i for i in range(24)]), ([2, 2, 1], [600, 2, 130])])
+def test_attend_rows_between_one_kernel_and_the_other(ql, kl, hd, heads, kv, dtype, q8):
+    """32 to 256 rows, where either kernel takes the batch, and up to 8, whose
+    weights are split whatever the type."""
+    import torch
+
+    c, batch = _cache(ql, kl, kv, hd, 48, q8, seed=sum(kl), poison=True)
+    q = torch.randn(batch.n_tokens, heads, hd, device="cuda").to(_dt(dtype)) * 2
+    for window in (0, 50):
+        out = c.attend(0, q, batch, window=window)
+        _clean()
+        _check_attend(c, 0, batch, q, out, window=window)
+
+
+def test_a_sequence_longer_than_stated_costs_only_itself():
+    """More new tokens than the max_q_len of the call (only a caller of the C
+    entry point can): that sequence's rows may stay, the others are right."""
+    import torch
+
+    from cybel_b200.paged_attention import RaggedBatch
+
+    for stated in (70, 3):
+        ql, kl = [300, stated, 2, 600], [900, 200, 300, 600]
+        c, batch = _cache(ql, kl, 2, 128, 64, False, seed=stated, poison=True)
+        q = torch.randn(batch.n_tokens, 8, 128, device="cuda").half()
+        batch.max_q = stated
+        out = torch.full_like(q, 9.0)
+        c.attend(0, q, batch, out=out)
+        _clean()
+        # (the others, checked alone: their rows and lengths in a batch of their own)
+        rest = [1, 2]
+        part = RaggedBatch([ql[b] for b in rest], [kl[b] for b in rest])
+        part.q_lens, part.kv_lens = [0] + part.q_lens, [0] + part.kv_lens
+        _check_attend(c, 0, part, q[300:], out[300:302 + stated])
