@@ -54,8 +54,7 @@ def rope(x, pos, freq, mag, half):
     return y
 
 
-def attention(q, k, v, pos, n, scale, cap=0.0, slopes=None, window=0, prefix=0, present=None,
-              k_rel=0.0, k_abs=0.0):
+def attention(q, k, v, pos, n, scale, cap=0.0, slopes=None, window=0, prefix=0, present=None):
     """q [rows][heads][hd] at positions pos [rows] over k, v [n][kv][hd]
     (values as stored): (out, bound) [rows][heads][hd] in float64.
 
@@ -64,7 +63,6 @@ def attention(q, k, v, pos, n, scale, cap=0.0, slopes=None, window=0, prefix=0, 
       d_j = scale sum|q||k| ((hd + 8) 2^-24 + 2^-22)   products, sums, split q
             + (|s_j| + |bias_j|) 2^-22                 scale, exponent argument
             + cap 2^-20                                tanh from exponentials,
-        + scale sum|q| (k_rel |k| + k_abs)         keys rounded on the way, if they are,
     and an output by sum_j p_j d_j (|v_j| + |out|), doubled for what is of
     second order. The roundings of the softmax weights and of the output are
     for the caller to add, relative to ``spread`` = sum_j p_j |v_j|, the third
@@ -91,7 +89,6 @@ def attention(q, k, v, pos, n, scale, cap=0.0, slopes=None, window=0, prefix=0, 
                 s = cap * np.tanh(s / cap)
             bias = slopes[h] * np.abs(i - js) if slopes is not None else np.zeros(len(js))
             d = mag * ((hd + 8) * 2.0 ** -24 + 2.0 ** -22) + (np.abs(s) + np.abs(bias)) * 2.0 ** -22 + cap * 2.0 ** -20
-            d = d + mag * k_rel + scale * np.abs(q[t, h]).sum() * k_abs
             s = s - bias
             p = np.exp(s - s.max())
             p /= p.sum()

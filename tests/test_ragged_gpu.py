@@ -10,11 +10,6 @@ Tolerances, per element, fixed before the kernels ran:
   (2^-11 relative in fp16; cached fp16 rows the same);
 * Q8 rows: the codes and scales are those of the exact rotation rounded to
   fp32 (the kernel rotates keys in fp64), compared for equality;
-* attention of fp16 rows over Q8 pages may take a key's or value's element as
-  code x scale rounded to fp16: 2^-11 of sum|q||k| scale on a score (weighed as
-  the oracle's bound weighs its own), 2^-11 of the spread on an output, and
-  2^-25 absolute per element below the smallest normal: scale sum|q| 2^-25 on a
-  score, 2^-25 on an output;
 * attention: oracle's bound for the scores, plus, relative to the spread
   sum_j p_j |v_j|, the rounding of the weights and of the sums: fp16 rows
   2^-11 for weights rounded to fp16 and 2^-11 for the output (2^-10 in all),
@@ -207,11 +202,8 @@ def _check_attend(c, layer, batch, q, got, scale=None, cap=0.0, slopes=None, win
             k, v, here = _rows64(c, layer, b, n)
             want, bound, spread = attention(
                 qn[at:at + m], k, v, np.arange(n - m, n), n, scale, cap, None if slopes is None else slopes,
-                window, 0 if prefix is None else prefix[b], here,
-                *((2.0 ** -11, 2.0 ** -25) if f16 and c.q8 else ()))
+                window, 0 if prefix is None else prefix[b], here)
             tol = bound + spread * (2.0 ** -10 + 2.0 ** -14 if f16 else 2.0 ** -19) + (2.0 ** -24 if f16 else 1e-30)
-            if f16 and c.q8:
-                tol = tol + spread * 2.0 ** -11 + 2.0 ** -25
             tol = tol + n * 2.0 ** -34 * np.abs(v[here], where=np.isfinite(v[here]), out=np.zeros_like(v[here])).max(initial=0)
             d = np.abs(got[at:at + m] - want)
             bad = ~(d <= tol)
