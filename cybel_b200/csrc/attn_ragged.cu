@@ -37,7 +37,7 @@ int few_rows(int batch, int n_kv, long long total_rows, int most, int max_kv, bo
     const double few_us = 3.0 + static_cast<double>(fw) * (6.0 + (fp32 ? 0.018 : 0.021) * max_kv / fc);
     const long long tu = tile_blocks(batch, total_rows, most, 32) * n_kv;
     const int tc = tile_split(tu, max_kv, sms);
-    const long long steps = (max_kv + 128 * tc - 1) / (128 * tc), tw = (tu * tc + sms - 1) / sms;
+    const long long steps = (max_kv + 128ll * tc - 1) / (128 * tc), tw = (tu * tc + sms - 1) / sms;
     const double step_us = fp32 ? (q8 ? 6.8 : 5.4) : (q8 ? 3.2 : 2.2);
     return few_us < (fp32 ? 16.0 : 11.0) + step_us * static_cast<double>(steps * tw) ? 256 : 32;
 }
