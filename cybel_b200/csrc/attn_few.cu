@@ -668,21 +668,20 @@ int launch_few(const AttnArgs& a0, int max_rows, int max_kv, int sms, cudaStream
 
 }  // namespace
 
+int few_slots(int sms) { return sms * kCtasPerSm; }
+
 // CTAs per block of rows: as many as one wave holds while the blocks leave SMs
 // idle, two where they fill more than half a wave (ragged lengths even out over
-// the halves), and 32 positions a warp at least. Measured at 4 x 8 rows of 2000
+// the halves), and about 64 positions a warp. Measured at 4 x 8 rows of 2000
 // positions: 17 us for one wave, 24 for two; 64 sequences of 100-8000: 191, 175,
-// 186 us for 1, 2, 4. Clusters of 16 for three quarters of a wave only: more of
-// them do not fit the GPCs (24 of them took 36 us at 8000 positions).
+// 186 us for 1, 2, 4. More than 8 only up to three quarters of a wave: larger
+// clusters do not fill the GPCs (24 of 16 took 36 us at 8000 positions, of 13 23).
 int few_split(long long units, int max_kv, int sms) {
-    const long long slots = static_cast<long long>(sms) * kCtasPerSm;
-    int c = 1;
-    while (c < kMaxCluster && (units * c * 2 <= (c * 2 < kMaxCluster ? slots : slots * 3 / 4) || c == 1) &&
-           max_kv > c * 2 * kWarps * 32)
-        c *= 2;
-    return c;
+    const long long slots = few_slots(sms);
+    long long c = std::max<long long>(slots / units, 2);
+    if (c > 8) c = std::max<long long>(8, std::min<long long>(kMaxCluster, slots * 3 / 4 / units));
+    return static_cast<int>(std::max<long long>(1, std::min<long long>(c, (max_kv + kWarps * 64 - 1) / (kWarps * 64))));
 }
-int few_slots(int sms) { return sms * kCtasPerSm; }
 
 int launch_attn_few(const AttnArgs& a, int hd, bool fp32, bool q8, int max_rows, int max_kv, int sms, cudaStream_t st) {
 #define B200Q_FEW3(D, FP32, SPLIT)                                             \

@@ -27,8 +27,8 @@ namespace {
 // few-row kernel's the positions of a CTA and its waves, the tile kernel's the
 // steps of a CTA, however full its tiles are. (24 tokens of 4 heads per kv head
 // at 2000 positions: fp32 26 against 35 us for 2 sequences, 50 against 52 for 4;
-// fp16 14 against 19 for 1, 29 against 25 for 4. Of 360 such batches six take
-// the kernel that is slower by more than 8 percent, by 33 at most.)
+// fp16 14 against 19 for 1, 29 against 25 for 4. Of 360 such batches two take
+// the kernel that is slower by more than 8 percent, by 20 at most.)
 int few_rows(int batch, int n_kv, long long total_rows, int most, int max_kv, bool fp32, bool q8, int sms) {
     if (most <= 32 || most > 256) return 32;
     const long long fu = static_cast<long long>(batch) * n_kv * ((most + (fp32 ? 7 : 15)) / (fp32 ? 8 : 16));
