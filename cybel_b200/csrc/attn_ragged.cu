@@ -23,14 +23,17 @@ namespace {
 // kernel is as fast or faster at any batch (8 tokens of 4 heads per kv head at
 // 2000 positions, fp16: 12 against 19 us for 1 sequence, 80 against 79 for 32).
 // Beyond, whichever comes out ahead by what their times follow, as measured at
-// 8 kv heads, 1 to 4 sequences of 48 to 256 rows and 300 to 8000 positions: the
+// 8 kv heads, 1 to 4 sequences of 48 to 256 rows and 300 to 8000 positions, and
+// at 1 to 8 kv heads with up to 4000 rows: the
 // few-row kernel's the positions of a CTA and its waves, the tile kernel's the
 // steps of a CTA, however full its tiles are. (24 tokens of 4 heads per kv head
 // at 2000 positions: fp32 26 against 35 us for 2 sequences, 50 against 52 for 4;
 // fp16 14 against 19 for 1, 29 against 25 for 4. Of 360 such batches two take
-// the kernel that is slower by more than 8 percent, by 20 at most.)
+// the kernel that is slower by more than 8 percent, by 20 at most. A prompt of
+// 600 tokens on one kv head, 4 heads, fp32: 21 against 34 us; of 128 tokens, 32/8
+// heads, fp16: 9 against 12; of 256: 17 against 14, the tile kernel's.)
 int few_rows(int batch, int n_kv, long long total_rows, int most, int max_kv, bool fp32, bool q8, int sms) {
-    if (most <= 32 || most > 256) return 32;
+    if (most <= 32) return 32;
     const long long fu = static_cast<long long>(batch) * n_kv * ((most + (fp32 ? 7 : 15)) / (fp32 ? 8 : 16));
     const int fc = few_split(fu, max_kv, sms);
     const long long fw = (fu * fc + few_slots(sms) - 1) / few_slots(sms);
@@ -39,7 +42,7 @@ int few_rows(int batch, int n_kv, long long total_rows, int most, int max_kv, bo
     const int tc = tile_split(tu, max_kv, sms);
     const long long steps = (max_kv + 128ll * tc - 1) / (128 * tc), tw = (tu * tc + sms - 1) / sms;
     const double step_us = fp32 ? (q8 ? 6.8 : 5.4) : (q8 ? 3.2 : 2.2);
-    return few_us < (fp32 ? 16.0 : 11.0) + step_us * static_cast<double>(steps * tw) ? 256 : 32;
+    return few_us < (fp32 ? 16.0 : 11.0) + step_us * static_cast<double>(steps * tw) ? most : 32;
 }
 
 }  // namespace
