@@ -364,7 +364,9 @@ __global__ void __launch_bounds__(kRopeThreads) b200q_rope_append_kernel(const A
     __shared__ double2 cs64[Q8 ? kMaxRows * 64 : 1];  // head <= 128
     __shared__ int2 place[kMaxRows];  // position and sequence of each row
     __shared__ uint32_t pool_of[kMaxRows];  // pool row of kv head 0 at the position; kNoRow without a page
-    griddep_launch_dependents();
+    // No early start for the kernels behind: the one-position attention reads the
+    // cached rows before it waits for the kernel ahead, and a kernel in between
+    // that passes its own start on would let it run beside this one's stores.
     griddep_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int np = a.s.rot / 2, hd = a.s.hd;
