@@ -89,6 +89,8 @@ SIGNATURES.update(
                                      _d, _i, _vp, _vp, _vp, _vp, _i, _i, _vp, _i, _vp], _i),
         "b200q_attention_paged": ([_vp, _i, _i, _i, _vp, _vp, _i, _i, _i, _i, _i, _ll, _vp, _ll, _f, _f, _vp, _i, _vp,
                                    _i, _vp, _vp, _vp, _vp, _i, _i, _vp, _i, _vp], _i),
+        "b200q_attention_paged_plan": ([_i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, ctypes.POINTER(ctypes.c_longlong),
+                                        _i], _i),
         "b200q_swiglu_q": ([_vp, _vp, _vp, _i, _i, _vp], _i),
         "b200q_swiglu_rows": ([_vp, _vp, _i, _i, _vp], _i),
         "b200q_matmul_xq": ([_i, _i, _vp, _vp, _vp, _i, _i, _i, ctypes.c_float, ctypes.c_float, _i, _vp], _i),

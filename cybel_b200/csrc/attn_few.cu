@@ -670,6 +670,8 @@ int launch_few(const AttnArgs& a0, int max_rows, int max_kv, int sms, cudaStream
 
 int few_slots(int sms) { return sms * kCtasPerSm; }
 
+int few_block_rows(bool fp32, int max_rows) { return fp32 || max_rows <= 8 ? 8 : 16; }
+
 // CTAs per block of rows: as many as one wave holds while the blocks leave SMs
 // idle, two where they fill more than half a wave (ragged lengths even out over
 // the halves), and about 64 positions a warp. Measured at 4 x 8 rows of 2000
@@ -687,7 +689,8 @@ int launch_attn_few(const AttnArgs& a, int hd, bool fp32, bool q8, int max_rows,
 #define B200Q_FEW3(D, FP32, SPLIT)                                             \
     (q8 ? launch_few<D, FP32, SPLIT, true>(a, max_rows, max_kv, sms, st) \
         : launch_few<D, FP32, SPLIT, false>(a, max_rows, max_kv, sms, st))
-#define B200Q_FEW(D) (fp32 ? B200Q_FEW3(D, true, true) : max_rows <= 8 ? B200Q_FEW3(D, false, true) : B200Q_FEW3(D, false, false))
+    const bool split = few_block_rows(fp32, max_rows) == 8;
+#define B200Q_FEW(D) (fp32 ? B200Q_FEW3(D, true, true) : split ? B200Q_FEW3(D, false, true) : B200Q_FEW3(D, false, false))
     return hd == 128 ? B200Q_FEW(128) : B200Q_FEW(64);
 #undef B200Q_FEW
 #undef B200Q_FEW3

@@ -45,6 +45,27 @@ int few_rows(int batch, int n_kv, long long total_rows, int most, int max_kv, bo
     return few_us < (fp32 ? 16.0 : 11.0) + step_us * static_cast<double>(steps * tw) ? most : 32;
 }
 
+// What a call launches, from its arguments alone.
+struct AttnPlan {
+    long long total_rows;
+    int most_rows;  // of a sequence
+    int few_rows;   // sequences of at most this many rows are the few-row kernel's
+    int reach;      // positions that a block of rows has to read, for the splits
+};
+
+AttnPlan attention_plan(bool fp32, bool q8, int n_tokens, int batch, int max_q_len, int max_kv_len, int heads, int n_kv,
+                        int window, bool prefix, int sms) {
+    AttnPlan p;
+    const int group = heads / n_kv, tokens = std::min(max_q_len, n_tokens);  // of a sequence
+    p.total_rows = static_cast<long long>(n_tokens) * group;                 // at most 2^30
+    p.most_rows = tokens * group;
+    p.reach = window > 0 && !prefix
+                  ? static_cast<int>(std::min<long long>(max_kv_len, static_cast<long long>(window) + tokens))
+                  : max_kv_len;
+    p.few_rows = few_rows(batch, n_kv, p.total_rows, p.most_rows, p.reach, fp32, q8, sms);
+    return p;
+}
+
 }  // namespace
 
 int launch_attention_paged(const void* q, int dtype, int n_tokens, int batch, const int* cu_q, const int* kv_len,
@@ -90,16 +111,33 @@ int launch_attention_paged(const void* q, int dtype, int n_tokens, int batch, co
     divisor(pkv.page_size, a.page_mul, a.page_shift);
     divisor(a.group, a.group_mul, a.group_shift);
     const bool q8 = pkv.kv_mode == B200Q_KV_Q8, fp32 = dtype == B200Q_F32;
-    const long long total_rows = static_cast<long long>(n_tokens) * a.group;  // at most 2^30
-    const int tokens = std::min(max_q_len, n_tokens);                        // of a sequence
-    a.most_rows = tokens * a.group;
-    // Positions that a row block has to read, for the splits below.
-    const int reach = window > 0 && !prefix ? static_cast<int>(std::min<long long>(max_kv_len, static_cast<long long>(window) + tokens))
-                                            : max_kv_len;
-    a.few_rows = few_rows(batch, pkv.n_kv, total_rows, a.most_rows, reach, fp32, q8, dev->num_sms);
-    rc = launch_attn_few(a, hd, fp32, q8, std::min(a.most_rows, a.few_rows), reach, dev->num_sms, st);
+    const AttnPlan p = attention_plan(fp32, q8, n_tokens, batch, max_q_len, max_kv_len, heads, pkv.n_kv, window,
+                                      prefix != nullptr, dev->num_sms);
+    a.most_rows = p.most_rows;
+    a.few_rows = p.few_rows;
+    rc = launch_attn_few(a, hd, fp32, q8, std::min(a.most_rows, a.few_rows), p.reach, dev->num_sms, st);
     if (rc != B200Q_OK || a.most_rows <= a.few_rows) return rc;
-    return launch_attn_tiles(a, hd, fp32, q8, total_rows, reach, dev->num_sms, st);
+    return launch_attn_tiles(a, hd, fp32, q8, p.total_rows, p.reach, dev->num_sms, st);
+}
+
+int attention_plan_info(int dtype, int n_tokens, int batch, int max_q_len, int max_kv_len, int heads, int n_kv,
+                        int window, bool prefix, int kv_mode, int num_sms, long long* out, int out_len) {
+    const bool q8 = kv_mode == B200Q_KV_Q8, fp32 = dtype == B200Q_F32;
+    if (!out || out_len < kAttnPlanFields || n_tokens <= 0 || batch <= 0 || max_q_len <= 0 || max_kv_len < 0 ||
+        heads <= 0 || n_kv <= 0 || window < 0 || num_sms <= 0 || (!fp32 && dtype != B200Q_F16) ||
+        (!q8 && kv_mode != B200Q_KV_F16))
+        return B200Q_EINVAL;
+    if (heads % n_kv || static_cast<long long>(n_tokens) * (heads / n_kv) > (1 << 30)) return B200Q_ESHAPE;
+    const AttnPlan p =
+        attention_plan(fp32, q8, n_tokens, batch, max_q_len, max_kv_len, heads, n_kv, window, prefix, num_sms);
+    const int few = std::min(p.most_rows, p.few_rows), rows = few_block_rows(fp32, few);
+    out[0] = p.few_rows;
+    out[1] = few_split(static_cast<long long>(batch) * n_kv * ((few + rows - 1) / rows), p.reach, num_sms);
+    const long long blocks =
+        p.most_rows > p.few_rows ? tile_blocks(batch, p.total_rows, p.most_rows, p.few_rows) * n_kv : 0;
+    out[2] = blocks;
+    out[3] = blocks > 0 ? tile_split(blocks, p.reach, num_sms) : 0;
+    return B200Q_OK;
 }
 
 }  // namespace b200q

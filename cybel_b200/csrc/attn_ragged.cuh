@@ -190,5 +190,7 @@ int tile_split(long long units, int max_kv, int sms);
 // The few-row kernel's split of `units` blocks, and the CTAs that run at once.
 int few_split(long long units, int max_kv, int sms);
 int few_slots(int sms);
+// Rows of its blocks, where no sequence has more than max_rows of its rows.
+int few_block_rows(bool fp32, int max_rows);
 
 }  // namespace b200q

@@ -1099,6 +1099,13 @@ int b200q_attention_paged(const void* q, int dtype, int n_tokens, int batch, con
     return rc;
 }
 
+int b200q_attention_paged_plan(int dtype, int n_tokens, int batch, int max_q_len, int max_kv_len, int n_heads,
+                               int n_kv_heads, int window, int prefix, int kv_mode, int num_sms, long long* out,
+                               int out_len) {
+    return attention_plan_info(dtype, n_tokens, batch, max_q_len, max_kv_len, n_heads, n_kv_heads, window, prefix != 0,
+                               kv_mode, num_sms, out, out_len);
+}
+
 // ---- controls ----------------------------------------------------------------
 int b200q_set_act_mode(int act_mode) {
     const int prev = act_mode_now();

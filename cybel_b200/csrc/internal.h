@@ -153,6 +153,10 @@ int launch_attention_paged(const void* q, int dtype, int n_tokens, int batch, co
                            int max_q_len, int max_kv_len, int heads, int hd, long long q_stride, void* out,
                            long long out_stride, float scale, float softcap, const float* slopes, int window,
                            const int* prefix, const PagedKV& pkv, Device* dev, cudaStream_t st);
+// What launch_attention_paged would launch (b200q_attention_paged_plan), as kAttnPlanFields values.
+constexpr int kAttnPlanFields = 4;
+int attention_plan_info(int dtype, int n_tokens, int batch, int max_q_len, int max_kv_len, int heads, int n_kv,
+                        int window, bool prefix, int kv_mode, int num_sms, long long* out, int out_len);
 int launch_swiglu(const float* g, const float* u, float* out, long long n, cudaStream_t st);
 // SiLU(gate) * up for `rows` rows of [gate n | up n] (b200q_swiglu_rows).
 int launch_swiglu_rows(const float* gu, float* out, int rows, int n, cudaStream_t st);

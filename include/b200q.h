@@ -425,6 +425,17 @@ B200Q_API int b200q_attention_paged(const void* q, int dtype, int n_tokens, int 
                                     const float* v_scales, int n_slots, int page_size, const int* page_table,
                                     int pages_per_seq, void* stream);
 
+/* What b200q_attention_paged launches for these arguments (prefix: whether one
+ * is given) on a device of num_sms SMs, without touching a device: out[0]
+ * the most rows (tokens x query heads per kv head) of a sequence that the
+ * few-row kernel takes, out[1] the CTAs that split its positions, out[2] the
+ * blocks of rows that the many-row kernel is launched for (0: not launched),
+ * out[3] the CTAs that split the positions of each. out_len >= 4. B200Q_OK,
+ * B200Q_EINVAL or B200Q_ESHAPE. */
+B200Q_API int b200q_attention_paged_plan(int dtype, int n_tokens, int batch, int max_q_len, int max_kv_len, int n_heads,
+                                         int n_kv_heads, int window, int prefix, int kv_mode, int num_sms,
+                                         long long* out, int out_len);
+
 B200Q_API int b200q_swiglu_q(const float* gate, const float* up, void* xq, int act_mode, int n, void* stream);
 /* out[r][j] = silu(gate_up[r][j]) * gate_up[r][n + j] for `rows` rows of one
  * gate|up projection output ([gate n | up n] per row): the SwiGLU step of a
