@@ -811,9 +811,18 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
 #pragma unroll
                         for (int u = 0; u < 4; ++u)
                             far[u] = max3(far[u], fabsf(x[c + 2 * u]), fabsf(x[c + 2 * u + 1]));
-                    if (__any_sync(0xffffffffu, fmaxf(fmaxf(far[0], far[1]), fmaxf(far[2], far[3])) > (PREC ? 1.0f : 0.5f))) {
+                    // Far arguments take the other form one by one: it is off by 2^-22 absolutely,
+                    // which the small scores beside them would feel (cap times as much).
+                    constexpr float kFar = PREC ? 1.0f : 0.5f;
+                    if (__any_sync(0xffffffffu, fmaxf(fmaxf(far[0], far[1]), fmaxf(far[2], far[3])) > kFar)) {
 #pragma unroll
-                        for (int c = 0; c < kRows; ++c) x[c] = tanh_far(x[c]);
+                        for (int c = 0; c < kRows; c += 2) {
+                            const float2 z = make_float2(x[c], x[c + 1]), near = tanh_near<PREC>(z);
+                            x[c] = fabsf(z.x) > kFar ? tanh_far(z.x) : near.x;
+                            x[c + 1] = fabsf(z.y) > kFar ? tanh_far(z.y) : near.y;
+                            // (four pairs at a time: all of them at once spill 300 to 500 bytes a thread)
+                            if ((c & 6) == 6) asm volatile("" ::: "memory");
+                        }
                     } else {
 #pragma unroll
                         for (int c = 0; c < kRows; c += 2) put2(x + c, tanh_near<PREC>(make_float2(x[c], x[c + 1])));

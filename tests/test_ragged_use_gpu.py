@@ -75,3 +75,146 @@ def test_one_position_attention_right_behind_an_append(q8, between):
         graph.replay()
         _clean()
         assert torch.equal(out, want)
+
+
+# ---- attention against the formula in 64 bits, all rows at once --------------------
+FEW = ([3, 1, 8, 0, 5], [300, 200, 333, 40, 128])
+MANY = ([700, 1, 600, 0, 700], [700, 40, 1000, 30, 900])  # blocks of both kernels, at any shape below
+
+
+def _plan(q, batch, kv, window=0, prefix=0, q8=False):
+    import torch
+
+    from tests.test_ragged_plan import plan
+
+    return plan("fp32" if q.dtype == torch.float32 else "fp16", batch.q_lens, batch.kv_lens, q.shape[1], kv, window, prefix, q8,
+                torch.cuda.get_device_properties(0).multi_processor_count)
+
+
+def _both(q, batch, kv, **kw):
+    """Whether a call launches both kernels."""
+    few, _, blocks, _ = _plan(q, batch, kv, **kw)
+    return blocks > 0 and max(batch.q_lens) * q.shape[1] // kv > few
+
+
+def _cache(lens, kv, hd, page, q8, seed, layers=1):
+    import torch
+
+    from cybel_b200.kv_cache import PagedKVCache
+    from cybel_b200.paged_attention import RaggedBatch
+
+    q_lens, kv_lens = lens
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    per = (max(kv_lens) + page - 1) // page
+    c = PagedKVCache(layers, kv, per * page, batch=len(kv_lens), page_size=page, q8=q8, head_dim=hd)
+    slots = torch.randperm(c.n_slots, generator=g, device="cuda").cpu().numpy().reshape(c.table_host.shape)
+    c.table_host[...] = slots
+    c.sync_table()
+    if q8:
+        for t in (c.k, c.v):
+            t.copy_(torch.randint(-127, 128, t.shape, generator=g, device="cuda", dtype=torch.int8))
+        for t in (c.ks, c.vs):
+            t.copy_(torch.rand(t.shape, generator=g, device="cuda") * 0.02 + 0.002)
+    else:
+        for t in (c.k, c.v):
+            t.copy_(torch.randn(t.shape, generator=g, device="cuda"))
+    return c, RaggedBatch(q_lens, kv_lens), g
+
+
+def _stored(c, layer, b, n):
+    """Keys and values of one sequence [kv][n][hd] in 64 bits."""
+    import torch
+
+    j = torch.arange(n, device="cuda")
+    slot = c.table[layer, b, j // c.page_size].long()
+    out = []
+    for t, s in ((c.k, c.ks), (c.v, c.vs)):
+        x = t[slot, :, j % c.page_size].double()
+        if s is not None:
+            x = x * s[slot, :, j % c.page_size].double()[..., None]
+        out.append(x.transpose(0, 1))
+    return out
+
+
+def _check(c, layer, batch, q, got, scale=None, cap=0.0, slopes=None, window=0, prefix=None, rows=None, terms=None):
+    """got against the formula in 64 bits. Tolerances are those of
+    test_ragged_gpu.py, with two terms taken by what they are: the products of
+    a score number `terms` (nonzero elements of a query row), and a cap moves
+    a score s by |s| 2^-20 in fp32 rows -- five factors and products of 2^-24
+    and tanh, 2^-24 below 1 and 2^-22 absolutely, hence 2^-21.6, above -- and
+    by |s| 2^-19 in fp16 rows, whose tanh is 2^-20.8. rows: those to look at."""
+    import torch
+
+    f16 = q.dtype == torch.float16
+    kv, hd = c.kv_heads, c.head_dim
+    heads = q.shape[1]
+    g = heads // kv
+    terms = hd if terms is None else terms
+    scale = hd ** -0.5 if scale is None else scale
+    at = 0
+    for b, (m, n) in enumerate(zip(batch.q_lens, batch.kv_lens)):
+        if not m:
+            continue
+        k, v = _stored(c, layer, b, n)
+        x = q[at:at + m].double().view(m, kv, g, hd).permute(1, 2, 0, 3)
+        s = scale * torch.einsum("agmd,and->agmn", x, k)
+        mag = scale * torch.einsum("agmd,and->agmn", x.abs(), k.abs())
+        pos, j = torch.arange(n - m, n, device="cuda")[:, None], torch.arange(n, device="cuda")[None, :]
+        if cap:
+            s = cap * torch.tanh(s / cap)
+        d = mag * ((terms + 8) * 2.0 ** -24 + 2.0 ** -22) + s.abs() * 2.0 ** -22
+        if cap:
+            d = d + s.abs() * (2.0 ** -19 if f16 else 2.0 ** -20)
+        if slopes is not None:
+            bias = slopes.double().view(kv, g, 1, 1) * (pos - j).abs()
+            s, d = s - bias, d + bias.abs() * 2.0 ** -22
+        see = (j <= pos) & ((pos - j < window) if window else True)
+        if prefix is not None:
+            see = see | (j < prefix[b])
+        s = s.masked_fill(~see, float("-inf"))
+        p = torch.softmax(s, -1)
+        p = torch.where(see.any(-1, keepdim=True), p, torch.zeros_like(p))
+        d = torch.where(see, d, torch.zeros_like(d))
+        want = torch.einsum("agmn,and->agmd", p, v)
+        spread = torch.einsum("agmn,and->agmd", p, v.abs())
+        bound = 2 * (torch.einsum("agmn,and->agmd", p * d, v.abs()) + (p * d).sum(-1, keepdim=True) * want.abs())
+        tol = bound + spread * (2.0 ** -10 + 2.0 ** -14 if f16 else 2.0 ** -19) + (2.0 ** -24 if f16 else 1e-30)
+        tol = tol + n * 2.0 ** -34 * v.abs().max()
+        flat = (lambda t: t.permute(2, 0, 1, 3).reshape(m, heads, hd))
+        diff = (got[at:at + m].double() - flat(want)).abs()
+        bad = ~(diff <= flat(tol))
+        if rows is not None:
+            bad &= rows[at:at + m].view(m, 1, 1)
+        assert not bad.any(), (b, bad.nonzero()[:4].tolist(), float((diff / flat(tol)).nan_to_num().max()), int(bad.sum()))
+        at += m
+
+
+def _one_hot(n, heads, hd, value, g):
+    """Query rows with one element each: a score is a single product."""
+    import torch
+
+    q = torch.zeros(n, heads, hd, device="cuda")
+    q.scatter_(2, torch.randint(0, hd, (n, heads, 1), generator=g, device="cuda"), value)
+    return q
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("dtype,cap,far", [("fp32", 50.0, 30000.0), ("fp32", 1000.0, 30000.0), ("fp16", 50.0, 60000.0),
+                                           ("fp16", 30000.0, 60000.0)])
+@pytest.mark.parametrize("hd,heads,kv", [(128, 8, 2), (64, 6, 2)])
+@pytest.mark.parametrize("lens", [FEW, MANY])
+def test_a_capped_row_does_not_depend_on_its_neighbours(lens, hd, heads, kv, dtype, cap, far, q8):
+    """Rows of small scores beside rows whose scores pass the cap: tanh of
+    each score is as exact as if it stood alone. (One-hot queries, whose
+    scores carry no error of a sum that would cover tanh's.)"""
+    import torch
+
+    c, batch, g = _cache(lens, kv, hd, 48, q8, seed=hd)
+    q = _one_hot(batch.n_tokens, heads, hd, 2.0, g)
+    q[::29] *= far / 2.0
+    q = q.to(torch.float32 if dtype == "fp32" else torch.float16)
+    assert lens is FEW or _both(q, batch, kv, q8=q8)
+    out = c.attend(0, q, batch, softcap=cap, scale=1.0)
+    _clean()
+    _check(c, 0, batch, q, out, scale=1.0, cap=cap, terms=1)
