@@ -475,15 +475,16 @@ __global__ void __launch_bounds__(kRopeThreads) b200q_rope_append_kernel(const A
         const int tasks = nr * nh * 2, step = 32 / lanes * (kRopeThreads / 32);
         for (int i0 = 0; i0 < tasks; i0 += step) {
             int i = i0 + warp * (32 / lanes) + sub;
-            const bool mine = i < tasks;
+            bool mine = i < tasks;
             i = mine ? i : 0;
             int r = 0;
             while (i >= 2 * nh) i -= 2 * nh, ++r;
+            mine = mine && pool_of[r] != kNoRow;  // a row of no sequence, or without a page, is not read
             const bool is_v = i >= nh;
             const int h = kh0 + (is_v ? i - nh : i);
             const T* src = static_cast<const T*>(is_v ? a.v : a.k) + (r0 + r) * a.kv_stride + h * hd;
-            float x[E], mate[E];
-            if (a.kv_wide) {
+            float x[E] = {}, mate[E] = {};
+            if (mine && a.kv_wide) {
                 Vec<T, E> v, w;
                 v.load(src + e0);
                 const bool other = !is_v && a.s.half && e0 < a.s.rot;
@@ -493,12 +494,11 @@ __global__ void __launch_bounds__(kRopeThreads) b200q_rope_append_kernel(const A
                     x[e] = v.get(e);
                     mate[e] = other ? w.get(e) : v.get(e ^ 1);
                 }
-            } else {
+            } else if (mine) {
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     const int el = e0 + e;
                     x[e] = load1(src + el);
-                    mate[e] = 0.0f;
                     if (!is_v && el < a.s.rot)
                         mate[e] = load1(src + (a.s.half ? (el < np ? el + np : el - np) : el ^ 1));
                 }
@@ -517,7 +517,7 @@ __global__ void __launch_bounds__(kRopeThreads) b200q_rope_append_kernel(const A
             }
             for (int o = lanes / 2; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
             const float scale = q8_scale(amax), inv = __fdiv_rn(1.0f, scale);
-            if (!mine || pool_of[r] == kNoRow) continue;
+            if (!mine) continue;
             const long long dst = pool_of[r] + static_cast<long long>(h) * a.kv.page;
             uint32_t lo = 0, up = 0;
 #pragma unroll

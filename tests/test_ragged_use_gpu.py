@@ -218,3 +218,36 @@ def test_a_capped_row_does_not_depend_on_its_neighbours(lens, hd, heads, kv, dty
     out = c.attend(0, q, batch, softcap=cap, scale=1.0)
     _clean()
     _check(c, 0, batch, q, out, scale=1.0, cap=cap, terms=1)
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("dtype", ["fp32", "fp16"])
+@pytest.mark.parametrize("half", [False, True])
+def test_rows_behind_the_last_sequence_take_no_part_in_an_append(half, dtype, q8):
+    """A batch updated to fewer tokens than its rows: what the rows behind
+    hold (here NaN) reaches nothing, and their queries stay as they were."""
+    import torch
+
+    from cybel_b200.paged_attention import RaggedBatch, RopeTable
+
+    lens = ([30, 2, 40], [60, 20, 200])
+    c, batch, g = _cache(lens, 2, 128, 16, q8, seed=4)
+    batch.update([3, 0, 10], [60, 20, 200])
+    n, used = batch.n_tokens, 13
+    rows = torch.randn(n, 8 * 128, generator=g, device="cuda").to(torch.float32 if dtype == "fp32" else torch.float16)
+    rows[used:] = float("nan")
+    q, k, v = (rows[:, a * 128:b * 128].view(n, b - a, 128) for a, b in ((0, 4), (4, 6), (6, 8)))
+    rope = RopeTable(128, layout="half" if half else "interleaved")
+    q_out = torch.full((n, 4, 128), 7.0, dtype=q.dtype, device="cuda")
+    pools = [t for t in (c.k, c.v, c.ks, c.vs) if t is not None]
+    before = [t.clone() for t in pools]
+    c.append(0, k, v, batch, rope=rope, q=q, q_out=q_out)
+    _clean()
+    assert (q_out[used:] == 7).all()
+    got = [t.clone() for t in pools]
+    short = RaggedBatch([3, 0, 10], [60, 20, 200])
+    for t, b in zip(pools, before):
+        t.copy_(b)
+    want = c.append(0, k[:used], v[:used], short, rope=rope, q=q[:used])
+    _clean()
+    assert torch.equal(q_out[:used], want) and all(torch.equal(a, b) for a, b in zip(got, pools))
