@@ -168,6 +168,6 @@ def check_device(device: int, what: str = "device status") -> None:
     if v < 0:
         raise NativeError(v, what)
     if v & STATUS_TIMEOUT:
-        raise NativeError(-7, what)
+        raise NativeError(-7, f"{what} ({STATUS[-11]}, too)" if v & STATUS_BAD_PAGE else what)
     if v & STATUS_BAD_PAGE:
         raise NativeError(-11, what)

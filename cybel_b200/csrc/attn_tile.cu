@@ -153,7 +153,7 @@ __device__ __forceinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatil
         if ((it & 7u) == 0u && global_timer_ns() - t0 > kWaitTimeoutNs) break;
     }
     *dead = 1;
-    *status = *status | STATUS_TIMEOUT;
+    *status = STATUS_TIMEOUT;
     return false;
 }
 struct Waiter {

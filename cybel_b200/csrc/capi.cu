@@ -1143,8 +1143,8 @@ int b200q_device_status(int device) {
     int v = noalloc_take_status(device);
     if (v < 0) return v;
     if (Device* d = device_state_if_present(device)) {
-        v |= *d->status_host;
-        *d->status_host = 0;
+        v |= d->status_host[0] | d->status_host[kBadPageWord];
+        d->status_host[0] = d->status_host[kBadPageWord] = 0;
     }
     return v;
 }

@@ -426,7 +426,7 @@ struct KvArgs {
     int page;             // positions per page
     int n_slots;          // pages in the pool
     int max_ctx;          // contiguous: positions per sequence
-    volatile int* status; // STATUS_BAD_PAGE is recorded here
+    volatile int* status; // STATUS_BAD_PAGE is recorded behind it
 };
 
 // Element offset of (sequence b, kv head h, position p) in the caches (the
@@ -441,7 +441,7 @@ __device__ __forceinline__ long long kv_row(const KvArgs& a, int b, int h, int n
     } else {
         const int slot = __ldg(a.table + static_cast<long long>(b) * a.pages_per_seq + p / a.page);
         if (slot < 0 || slot >= a.n_slots) {
-            if (slot >= a.n_slots) *a.status = STATUS_BAD_PAGE;
+            if (slot >= a.n_slots) a.status[kBadPageWord] = STATUS_BAD_PAGE;
             return -1;
         }
         return ((static_cast<long long>(slot) * n_kv + h) * a.page + (p % a.page)) * kHeadDim;
@@ -665,7 +665,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 2) b200q_attn_decode_kernel(
     if (c == n_chunks - 1) {  // this chunk holds my_pos: append its rotated key and value
         const long long prow = kv_row<KVM>(kv, seq, kvh, n_kv, my_pos);
         if (prow < 0) {
-            if (threadIdx.x == 0) *kv.status = STATUS_BAD_PAGE;  // no page to append to
+            if (threadIdx.x == 0) kv.status[kBadPageWord] = STATUS_BAD_PAGE;  // no page to append to
         } else if (warp < 2) {  // warp 0: the key, warp 1: the value (lane l: elements 4l .. 4l+3)
             const float* src = (warp == 0 ? k_seq : v_seq) + tok * tok_stride;
             const float4 x = warp == 0 ? rope_lane(src, my_pos, lane, log2_theta)

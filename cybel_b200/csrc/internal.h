@@ -24,7 +24,7 @@ long long row_bytes_of(int qtype, int k);
 struct Device {
     int id = -1;
     int num_sms = 0;
-    volatile int* status_host = nullptr;  // host view of the mapped status word
+    volatile int* status_host = nullptr;  // host view of the mapped status words
     volatile int* status = nullptr;       // device view (kernels write STATUS_* values)
 };
 Device* device_state(int dev, int* err);

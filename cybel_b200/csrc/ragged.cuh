@@ -87,7 +87,7 @@ __device__ __forceinline__ int page_slot(const PagedView& kv, int b, int pg) {
 }
 
 __device__ __forceinline__ void flag_bad_page(const PagedView& kv) {
-    *kv.status = *kv.status | STATUS_BAD_PAGE;
+    kv.status[kBadPageWord] = STATUS_BAD_PAGE;
 }
 
 // Row index (of hd elements, or of one scale) of position `off` of a page.
