@@ -72,9 +72,9 @@ int launch_attention_paged(const void* q, int dtype, int n_tokens, int batch, co
                            int max_q_len, int max_kv_len, int heads, int hd, long long q_stride, void* out,
                            long long out_stride, float scale, float softcap, const float* slopes, int window,
                            const int* prefix, const PagedKV& pkv, Device* dev, cudaStream_t st) {
-    if (!q || !out || !cu_q || !kv_len || n_tokens < 0 || batch <= 0 || heads <= 0 || max_q_len < 0 || max_kv_len < 0 ||
-        !dev)
+    if (!cu_q || !kv_len || n_tokens < 0 || batch <= 0 || heads <= 0 || max_q_len < 0 || max_kv_len < 0 || !dev)
         return B200Q_EINVAL;
+    if (n_tokens > 0 && (!q || !out)) return B200Q_EINVAL;  // (rows of no memory have no address)
     if (dtype != B200Q_F32 && dtype != B200Q_F16) return B200Q_EINVAL;
     if (!(scale > 0.0f) || !std::isfinite(scale) || !(softcap >= 0.0f) || !std::isfinite(softcap) || window < 0)
         return B200Q_EINVAL;

@@ -620,7 +620,8 @@ int rope_table(int rot_dim, double theta, int scaling, double factor, double low
 int launch_rope_rows(const void* x, void* out, int dtype, int rows, int heads, int hd, long long x_stride,
                      long long out_stride, const int* positions, const unsigned long long* turns, int rot, int layout,
                      double mag, Device* dev, cudaStream_t st) {
-    if (!x || !out || !positions || !turns || rows < 0 || heads <= 0 || hd <= 0 || !dev) return B200Q_EINVAL;
+    if (!turns || rows < 0 || heads <= 0 || hd <= 0 || !dev) return B200Q_EINVAL;
+    if (rows > 0 && (!x || !out || !positions)) return B200Q_EINVAL;  // (rows of no memory have no address)
     if ((dtype != B200Q_F32 && dtype != B200Q_F16) || (layout != B200Q_ROPE_INTERLEAVED && layout != B200Q_ROPE_HALF))
         return B200Q_EINVAL;
     if (rot <= 0 || rot % 2 || rot > hd || rot > kMaxRot) return B200Q_ESHAPE;
@@ -700,7 +701,8 @@ int launch_rope_append(const void* q, const void* k, const void* v, int dtype, i
                        const int* kv_len, int heads, int hd, long long q_stride, long long kv_stride, void* q_out,
                        long long q_out_stride, const unsigned long long* turns, int rot, int layout, double mag,
                        const PagedKV& pkv, Device* dev, cudaStream_t st) {
-    if (!k || !v || !cu_q || !kv_len || n_tokens < 0 || batch <= 0 || !dev) return B200Q_EINVAL;
+    if (!cu_q || !kv_len || n_tokens < 0 || batch <= 0 || !dev) return B200Q_EINVAL;
+    if (n_tokens > 0 && (!k || !v)) return B200Q_EINVAL;  // (rows of no memory have no address)
     if (q_out && (!q || heads <= 0)) return B200Q_EINVAL;
     if (dtype != B200Q_F32 && dtype != B200Q_F16) return B200Q_EINVAL;
     if (turns && layout != B200Q_ROPE_INTERLEAVED && layout != B200Q_ROPE_HALF) return B200Q_EINVAL;

@@ -364,7 +364,8 @@ B200Q_API int b200q_rope_attention_decode_paged(const float* q, const float* k, 
  * kv_len[b] - q_len + t). cu_q ([batch + 1], not falling) and kv_len ([batch])
  * are device int32 arrays that only the kernels read, so a captured graph
  * replays with the lengths they hold then. Rows that cu_q gives to no
- * sequence are neither read nor written; a sequence may have no rows.
+ * sequence are neither read nor written; a sequence may have no rows, and a
+ * call may have none at all (its row pointers may be NULL then).
  * Strides count elements between consecutive rows (0: packed). The paged
  * cache is that of b200q_rope_attention_decode_paged, head_dim 64 or 128.
  * ------------------------------------------------------------------- */

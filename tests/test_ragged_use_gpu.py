@@ -251,3 +251,26 @@ def test_rows_behind_the_last_sequence_take_no_part_in_an_append(half, dtype, q8
     want = c.append(0, k[:used], v[:used], short, rope=rope, q=q[:used])
     _clean()
     assert torch.equal(q_out[:used], want) and all(torch.equal(a, b) for a, b in zip(got, pools))
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("dtype", ["fp32", "fp16"])
+def test_a_step_without_new_tokens(dtype, q8):
+    """No sequence has a token this time (rows of no memory at all): the calls
+    do nothing, a new tensor has no rows, the cache keeps what it holds."""
+    import torch
+
+    from cybel_b200.paged_attention import RaggedBatch, RopeTable
+
+    c, _, _ = _cache(([1, 1], [30, 20]), 2, 128, 16, q8, seed=1)
+    batch = RaggedBatch([0, 0], [30, 20])
+    rows = (lambda h: torch.empty(0, h, 128, dtype=torch.float32 if dtype == "fp32" else torch.float16, device="cuda"))
+    rope = RopeTable(128)
+    before = c.k.clone()
+    c.ensure_batch(batch)
+    assert c.append(0, rows(2), rows(2), batch, rope=rope, q=rows(4)).shape == (0, 4, 128)
+    assert c.append(0, rows(2), rows(2), batch) is None
+    assert c.attend(0, rows(4), batch, window=3).shape == (0, 4, 128)
+    assert rope.rotate(rows(4), torch.empty(0, dtype=torch.int32, device="cuda")).shape == (0, 4, 128)
+    _clean()
+    assert torch.equal(c.k, before)
