@@ -146,6 +146,17 @@ def lib() -> ctypes.CDLL:
     return _LIB
 
 
+def torch_device(device):
+    """The torch device of a CUDA ordinal or a device string, with the current
+    device's ordinal where a CUDA device is named without one."""
+    import torch
+
+    dev = torch.device("cuda", device) if isinstance(device, int) else torch.device(device)
+    if dev.type == "cuda" and dev.index is None:
+        dev = torch.device("cuda", torch.cuda.current_device())
+    return dev
+
+
 def check(status: int, what: str) -> None:
     if int(status) != 0:
         raise NativeError(status, what)

@@ -85,7 +85,7 @@ class PagedKVCache:
         self.n_slots = full if n_slots is None else int(n_slots)
         if self.n_slots <= 0:
             raise ValueError("n_slots must be positive")
-        self.dev = torch.device("cuda", device) if isinstance(device, int) else torch.device(device)
+        self.dev = _native.torch_device(device)
         shape = (self.n_slots, kv_heads, page_size, head_dim)
         dt = torch.int8 if self.q8 else torch.float16
         self.k = torch.zeros(shape, dtype=dt, device=self.dev)

@@ -27,13 +27,6 @@ import torch
 from . import _native
 
 
-def _cuda_index(device):
-    dev = torch.device("cuda", device) if isinstance(device, int) else torch.device(device)
-    if dev.type == "cuda" and dev.index is None:
-        dev = torch.device("cuda", torch.cuda.current_device())
-    return dev
-
-
 class RopeTable:
     """Rotary frequencies of the first ``rot_dim`` elements of a head.
 
@@ -65,7 +58,7 @@ class RopeTable:
             turns.ctypes.data_as(ctypes.POINTER(ctypes.c_ulonglong)), ctypes.byref(mag)), "rotary table")
         self.rot_dim, self.layout, self.mag = rot_dim, layout, mag.value
         self.turns_host = turns
-        self.dev = _cuda_index(device)
+        self.dev = _native.torch_device(device)
         self.turns = torch.from_numpy(turns.view(np.int64)).to(self.dev)
         self._ptr, self._layout = self.turns.data_ptr(), _native.ROPE_LAYOUTS[layout]
         self._index = device_index(self.dev)
@@ -101,7 +94,7 @@ class RaggedBatch:
     a batch that grows is made with."""
 
     def __init__(self, q_lens, kv_lens, device: int | str = 0, max_q: int | None = None, max_kv: int | None = None):
-        self.dev = _cuda_index(device)
+        self.dev = _native.torch_device(device)
         self._index = device_index(self.dev)
         q, kv = self._checked(q_lens, kv_lens)
         self.batch, self.n_tokens = len(q), sum(q)

@@ -274,3 +274,23 @@ def test_a_step_without_new_tokens(dtype, q8):
     assert rope.rotate(rows(4), torch.empty(0, dtype=torch.int32, device="cuda")).shape == (0, 4, 128)
     _clean()
     assert torch.equal(c.k, before)
+
+
+def test_a_cache_on_the_current_device_by_name():
+    """device="cuda" (a torch device string without an ordinal) is the
+    current device, for the cache as for the tables and batches."""
+    import torch
+
+    from cybel_b200.kv_cache import PagedKVCache
+    from cybel_b200.paged_attention import RaggedBatch, RopeTable
+
+    c = PagedKVCache(1, 1, 32, batch=1, page_size=16, q8=False, device="cuda")
+    batch = RaggedBatch([2], [2], device="cuda")
+    c.ensure_batch(batch)
+    x = torch.ones(2, 1, 128, device="cuda")
+    q = c.append(0, x, x, batch, rope=RopeTable(128, device="cuda"), q=x)
+    assert torch.equal(c.attend(0, q, batch), x)
+    view = PagedKVCache.over_contiguous(*(torch.zeros(1, 1, 32, 128, dtype=torch.float16, device="cuda") for _ in range(2)))
+    view.append(0, x, x, batch)
+    assert torch.equal(view.attend(0, q, batch), x)
+    _clean()
