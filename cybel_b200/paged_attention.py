@@ -26,6 +26,8 @@ import torch
 
 from . import _native
 
+_INT_MAX = 2 ** 31 - 1  # of the C entry points' ints, past which ctypes cuts numbers off
+
 
 class RopeTable:
     """Rotary frequencies of the first ``rot_dim`` elements of a head.
@@ -49,6 +51,8 @@ class RopeTable:
             raise ValueError(f"unknown rotary scaling {scaling!r}")
         if rot_dim <= 0 or rot_dim % 2 or rot_dim > 256:
             raise ValueError("rot_dim must be even and at most 256")
+        if not 0 <= original_context <= _INT_MAX:
+            raise ValueError("original_context out of range")
         low = 1.0 if low is None else float(low)
         high = (32.0 if scaling == "yarn" else 4.0) if high is None else float(high)
         turns = np.empty(rot_dim // 2, dtype=np.uint64)
@@ -98,7 +102,7 @@ class RaggedBatch:
         self._index = device_index(self.dev)
         q, kv = self._checked(q_lens, kv_lens)
         self.batch, self.n_tokens = len(q), sum(q)
-        self.max_q = max(q) if max_q is None else int(max_q)
+        self.max_q = max(q) if max_q is None else min(int(max_q), self.n_tokens)  # (of all rows at most)
         self.max_kv = max(kv) if max_kv is None else int(max_kv)
         self.cu_q = torch.empty(self.batch + 1, dtype=torch.int32, device=self.dev)
         self.kv_len = torch.empty(self.batch, dtype=torch.int32, device=self.dev)
@@ -252,8 +256,10 @@ def attend(cache, layer, q, batch, out=None, scale=None, softcap=0.0, slopes=Non
     if prefix is not None:
         _vector(prefix, "prefix", torch.int32, batch.batch, index)
         prefix = prefix.data_ptr()
+    if window < 0:
+        raise ValueError("window must not be negative")
     _call(index, _native.lib().b200q_attention_paged, "paged attention", q.data_ptr(), dt, n, batch.batch,
           batch.cu_q.data_ptr(), batch.kv_len.data_ptr(), batch.max_q, batch.max_kv, heads, cache.kv_heads, hd, qs,
-          out.data_ptr(), os_, 1.0 / math.sqrt(hd) if scale is None else scale, softcap, slopes, window, prefix,
-          *cache._pools(layer))
+          out.data_ptr(), os_, 1.0 / math.sqrt(hd) if scale is None else scale, softcap, slopes, min(window, _INT_MAX),
+          prefix, *cache._pools(layer))
     return out

@@ -294,3 +294,15 @@ def test_a_cache_on_the_current_device_by_name():
     view.append(0, x, x, batch)
     assert torch.equal(view.attend(0, q, batch), x)
     _clean()
+
+
+@pytest.mark.parametrize("lens", [FEW, MANY])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 32 + 5])
+def test_a_window_past_every_length_is_none(lens, window):
+    import torch
+
+    c, batch, g = _cache(lens, 2, 128, 48, False, seed=2)
+    q = torch.randn(batch.n_tokens, 8, 128, generator=g, device="cuda").half()
+    assert lens is FEW or _both(q, batch, 2)
+    assert torch.equal(c.attend(0, q, batch, window=window), c.attend(0, q, batch))
+    _clean()
