@@ -131,6 +131,10 @@ __global__ void b200q_dequant_rows_kernel(int qtype, const uint8_t* __restrict__
     if (i >= static_cast<long long>(nrows) * k) return;
     const int r = static_cast<int>(i / k), c = static_cast<int>(i % k);
     const int row = rows[r];
+    if (tail_canonical && static_cast<unsigned>(row) >= static_cast<unsigned>(n)) {  // (n counts the matrix' rows then)
+        out[i] = __int_as_float(0x7FFFFFFF);  // NaN: there is no such row
+        return;
+    }
     const int b = c / elems, e = c % elems;
     const long long rb = static_cast<long long>(k / elems) * bbytes;
     long long off;

@@ -117,6 +117,24 @@ def random_rows(qtype: int, n: int, k: int, rng: np.random.Generator, block_rows
     return np.ascontiguousarray(np.tile(blk, (reps, 1))[:n])
 
 
+def prompt_ids(tokens, vocab: int):
+    """``tokens`` (integers, or an integer tensor [n]) as an int32 tensor [n]
+    where they are. Raises ValueError when there are none, or one that is
+    not a row of the embedding (a tensor on the device is read back for that)."""
+    import torch
+
+    if not isinstance(tokens, torch.Tensor):
+        tokens = torch.tensor([int(t) for t in tokens], dtype=torch.int64)
+    if tokens.dim() != 1 or tokens.is_floating_point() or tokens.is_complex() or tokens.dtype is torch.bool:
+        raise ValueError("tokens must be a row of integers")
+    if not tokens.numel():
+        raise ValueError("no tokens to prefill")
+    lo, hi = (int(x) for x in torch.aminmax(tokens))
+    if lo < 0 or hi >= vocab:
+        raise ValueError(f"a token outside the vocabulary of {vocab}")
+    return tokens.to(torch.int32)
+
+
 @dataclass
 class _Layer:
     wqkv: DeviceMatrix      # q, k and v rows, one after the other
@@ -325,15 +343,16 @@ class DecodeStack:
         over the cache in two launches per layer
         (b200q_rope_append_paged, b200q_attention_paged), and only the last
         row meets the LM head. Works on any of the stack's caches. ``tokens``:
-        integers, or an integer tensor."""
+        integers of the vocabulary, or an integer tensor of them."""
         import torch
 
         from .kv_cache import PagedKVCache
         from .paged_attention import RaggedBatch, RopeTable
 
-        n = len(tokens)
-        if n <= 0 or chunk <= 0:
+        if chunk <= 0:
             raise ValueError("no tokens to prefill")
+        ids = prompt_ids(tokens, self.shape.vocab)
+        n = ids.numel()
         if pos0 < 0 or pos0 + n > self.max_ctx:
             raise ValueError("positions outside the KV cache")
         s, L = self.shape, self.lib
@@ -343,8 +362,7 @@ class DecodeStack:
                 cache = PagedKVCache.over_contiguous(self.k_cache, self.v_cache)
             self._prompt = (cache, RopeTable(s.head_dim, s.rope_theta, device=self.dev.index))
         cache, rope = self._prompt
-        ids = tokens if isinstance(tokens, torch.Tensor) else torch.tensor([int(t) for t in tokens])
-        ids = ids.to(device=self.dev, dtype=torch.int32)
+        ids = ids.to(self.dev).contiguous()
         if self.kv_cache is not None:
             cache.ensure(pos0, pos0 + n - 1)
         act, W = self.act_mode, _native.WEIGHTS_STATIC | _native.TILE_FROM_2

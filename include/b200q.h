@@ -229,7 +229,8 @@ B200Q_API int b200q_matvec_noalloc(int qtype, int act_mode, const float* x, cons
 B200Q_API int b200q_repack(int dst_qtype, const void* src, void* dst, int k, int n, void* stream);
 
 /* out[i][k] = dequantized row rows[i] (device int array) of a matrix with n
- * rows; the R4 tail rows are addressed canonically (QM:2179-2296 values). */
+ * rows; the R4 tail rows are addressed canonically (QM:2179-2296 values).
+ * An index outside [0, n) reads nothing and gives a row of NaN. */
 B200Q_API int b200q_dequantize_rows(int qtype, const void* w, const int* rows, int nrows, float* out, int k, int n,
                                     void* stream);
 
