@@ -415,7 +415,9 @@ B200Q_API int b200q_rope_append_paged(const void* q, const void* k, const void* 
  * or NULL). Pages that no row sees need not be assigned (entry -1); an entry
  * outside the pool, or a visible position past the table, hides the position
  * and sets device status bit 2. A row that sees nothing is written as zeros.
- * Non-finite keys or values reach only the rows that see them. max_q_len and
+ * Non-finite keys or values reach only the rows that see them; where that
+ * leaves a score of -infinity the position has no weight, but fp32 rows may be
+ * NaN for an infinite key element (their queries have two parts). max_q_len and
  * max_kv_len, upper bounds of the sequences' rows and of kv_len, choose the
  * kernel and how the keys are split; a sequence with more rows than max_q_len
  * may be left unwritten. out may be q. scale > 0. q and out 16-byte aligned, strides a multiple of 16 bytes. */

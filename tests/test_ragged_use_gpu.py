@@ -123,27 +123,30 @@ def _cache(lens, kv, hd, page, q8, seed, layers=1):
 
 
 def _stored(c, layer, b, n):
-    """Keys and values of one sequence [kv][n][hd] in 64 bits."""
+    """Keys and values of one sequence [kv][n][hd] in 64 bits, the keys as
+    they lie and their factors [kv][n] apart (a Q8 score is the product of the
+    codes times the scale)."""
     import torch
 
     j = torch.arange(n, device="cuda")
-    slot = c.table[layer, b, j // c.page_size].long()
-    out = []
-    for t, s in ((c.k, c.ks), (c.v, c.vs)):
-        x = t[slot, :, j % c.page_size].double()
-        if s is not None:
-            x = x * s[slot, :, j % c.page_size].double()[..., None]
-        out.append(x.transpose(0, 1))
-    return out
+    slot, off = c.table[layer, b, j // c.page_size].long(), j % c.page_size
+    get = (lambda t: t[slot, :, off].double().transpose(0, 1))
+    k, v = get(c.k), get(c.v)
+    if c.ks is None:
+        return k, torch.ones_like(k[..., 0]), v
+    return k, get(c.ks), v * get(c.vs)[..., None]
 
 
-def _check(c, layer, batch, q, got, scale=None, cap=0.0, slopes=None, window=0, prefix=None, rows=None, terms=None):
-    """got against the formula in 64 bits. Tolerances are those of
-    test_ragged_gpu.py, with two terms taken by what they are: the products of
-    a score number `terms` (nonzero elements of a query row), and a cap moves
-    a score s by |s| 2^-20 in fp32 rows -- five factors and products of 2^-24
-    and tanh, 2^-24 below 1 and 2^-22 absolutely, hence 2^-21.6, above -- and
-    by |s| 2^-19 in fp16 rows, whose tanh is 2^-20.8. rows: those to look at."""
+def _check(c, layer, batch, q, got, scale=None, cap=0.0, slopes=None, window=0, prefix=None, terms=None):
+    """got against the formula in 64 bits; returns the tolerances. They are
+    those of test_ragged_gpu.py, with two terms taken by what they are: the
+    products of a score number `terms` (nonzero elements of a query row), and a
+    cap moves a score s by |s| 2^-20 in fp32 rows -- five factors and products
+    of 2^-24 and tanh, 2^-24 below 1 and 2^-22 absolutely, hence 2^-21.6, above
+    -- and by |s| 2^-19 in fp16 rows, whose tanh is 2^-20.8. A value that is not
+    finite is added to the rows that give it a weight, as a product with that
+    weight is; a row whose formula gives NaN or an infinity has to give it, and
+    an fp32 row that sees an infinite element of a key may give NaN."""
     import torch
 
     f16 = q.dtype == torch.float16
@@ -152,14 +155,16 @@ def _check(c, layer, batch, q, got, scale=None, cap=0.0, slopes=None, window=0, 
     g = heads // kv
     terms = hd if terms is None else terms
     scale = hd ** -0.5 if scale is None else scale
-    at = 0
+    at, tols = 0, torch.zeros(q.shape, dtype=torch.float64, device="cuda")
     for b, (m, n) in enumerate(zip(batch.q_lens, batch.kv_lens)):
         if not m:
             continue
-        k, v = _stored(c, layer, b, n)
+        k, ks, v = _stored(c, layer, b, n)
+        odd = ~torch.isfinite(v)
+        fine = v.masked_fill(odd, 0.0)
         x = q[at:at + m].double().view(m, kv, g, hd).permute(1, 2, 0, 3)
-        s = scale * torch.einsum("agmd,and->agmn", x, k)
-        mag = scale * torch.einsum("agmd,and->agmn", x.abs(), k.abs())
+        s = scale * torch.einsum("agmd,and->agmn", x, k) * ks[:, None, None, :]
+        mag = scale * torch.einsum("agmd,and->agmn", x.abs(), k.abs()) * ks.abs()[:, None, None, :]
         pos, j = torch.arange(n - m, n, device="cuda")[:, None], torch.arange(n, device="cuda")[None, :]
         if cap:
             s = cap * torch.tanh(s / cap)
@@ -175,19 +180,25 @@ def _check(c, layer, batch, q, got, scale=None, cap=0.0, slopes=None, window=0, 
         s = s.masked_fill(~see, float("-inf"))
         p = torch.softmax(s, -1)
         p = torch.where(see.any(-1, keepdim=True), p, torch.zeros_like(p))
-        d = torch.where(see, d, torch.zeros_like(d))
-        want = torch.einsum("agmn,and->agmd", p, v)
-        spread = torch.einsum("agmn,and->agmd", p, v.abs())
-        bound = 2 * (torch.einsum("agmn,and->agmd", p * d, v.abs()) + (p * d).sum(-1, keepdim=True) * want.abs())
+        d = torch.where(p > 0, d, torch.zeros_like(d))
+        want = torch.einsum("agmn,and->agmd", p, fine)
+        spread = torch.einsum("agmn,and->agmd", p, fine.abs())
+        bound = 2 * (torch.einsum("agmn,and->agmd", p * d, fine.abs()) + (p * d).sum(-1, keepdim=True) * want.abs())
+        for a, jj in odd.any(-1).nonzero().tolist():
+            extra = torch.where(odd[a, jj], v[a, jj], torch.zeros_like(v[a, jj]))
+            want[a] += torch.where((p[a, :, :, jj] > 0)[..., None], extra, torch.zeros_like(extra))
         tol = bound + spread * (2.0 ** -10 + 2.0 ** -14 if f16 else 2.0 ** -19) + (2.0 ** -24 if f16 else 1e-30)
-        tol = tol + n * 2.0 ** -34 * v.abs().max()
+        tol = tol + n * 2.0 ** -34 * fine.abs().max()
         flat = (lambda t: t.permute(2, 0, 1, 3).reshape(m, heads, hd))
-        diff = (got[at:at + m].double() - flat(want)).abs()
-        bad = ~(diff <= flat(tol))
-        if rows is not None:
-            bad &= rows[at:at + m].view(m, 1, 1)
-        assert not bad.any(), (b, bad.nonzero()[:4].tolist(), float((diff / flat(tol)).nan_to_num().max()), int(bad.sum()))
+        want, tol = flat(want), flat(tol)
+        mine = got[at:at + m].double()
+        diff = (mine - want).abs()
+        free = (torch.isinf(k).any(-1)[:, None, None, :] & see).any(-1) & (not f16)
+        good = (mine.isnan() & flat(free[..., None].expand(kv, g, m, hd))) | torch.where(torch.isfinite(want), diff <= tol, (mine == want) | (mine.isnan() & want.isnan()))
+        assert good.all(), (b, (~good).nonzero()[:4].tolist(), float((diff / tol).nan_to_num().max()), int((~good).sum()))
+        tols[at:at + m] = tol
         at += m
+    return tols
 
 
 def _one_hot(n, heads, hd, value, g):
