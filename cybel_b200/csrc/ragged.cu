@@ -5,7 +5,8 @@
 // the product loses the phase of far positions (at pos = 1e6 its last bit is
 // 0.06 rad), so the table holds f_p / (2 pi) as a 64-bit fraction of a turn
 // and the kernels form pos * turn modulo 2^64: the whole turns drop out of
-// the product exactly and what is left is off by at most pos * 2^-65 turns.
+// the product exactly and what is left is off by at most pos * 2^-63 turns
+// (the table's rounding, and that of the 64-bit mantissas it is computed in).
 // The fraction's nearest quarter turn is taken out as an integer too, so that
 // sincospi sees at most an eighth of a turn, with all 24 bits of it.
 //
@@ -104,8 +105,8 @@ __device__ __forceinline__ float2 cos_sin(int pos, uint64_t turn, float mag) {
     return (quarter & 2u) ? make_float2(-cc * mag, -ss * mag) : make_float2(cc * mag, ss * mag);
 }
 // The same in fp64, by the Taylor series about 0: an eighth of a turn is
-// pi / 4 at most, where the first terms left out are below 2^-56 (sin: x^17 /
-// 17!, cos: x^18 / 18!).
+// pi / 4 at most, where the first terms left out are below 2^-54 (sin: x^17 /
+// 17!) and 2^-58 (cos: x^18 / 18!).
 __device__ __forceinline__ double2 cos_sin64(int pos, uint64_t turn, double mag) {
     const uint64_t a = static_cast<uint64_t>(static_cast<uint32_t>(pos)) * turn;
     const uint64_t quarter = (a + (1ull << 61)) >> 62;
@@ -584,34 +585,35 @@ int rope_table(int rot_dim, double theta, int scaling, double factor, double low
     if (scaling != B200Q_ROPE_PLAIN && !(factor >= 1.0 && std::isfinite(factor))) return B200Q_EINVAL;
     const bool bands = scaling == B200Q_ROPE_LLAMA3 || scaling == B200Q_ROPE_YARN;
     if (bands && (original_context <= 0 || !(low > 0.0) || !(high > low) || !std::isfinite(high))) return B200Q_EINVAL;
-    const double two_pi = 6.283185307179586476925286766559;
+    const long double two_pi = 6.283185307179586476925286766559L;
     double y_lo = 0.0, y_hi = 1.0;
     if (scaling == B200Q_ROPE_YARN) {
         // the pair whose frequency makes beta turns over the original context
         auto at = [&](double beta) {
-            return rot_dim * std::log(original_context / (beta * two_pi)) / (2.0 * std::log(theta));
+            return static_cast<double>(rot_dim * std::log(original_context / (beta * two_pi)) /
+                                       (2.0L * std::log(static_cast<long double>(theta))));
         };
         y_lo = std::max(0.0, std::floor(at(high)));
         y_hi = std::min(rot_dim - 1.0, std::ceil(at(low)));
         if (!(y_hi > y_lo)) y_hi = y_lo + 0.001;
     }
     for (int p = 0; p < rot_dim / 2; ++p) {
-        double f = std::pow(theta, -2.0 * p / rot_dim);
+        long double f = std::pow(static_cast<long double>(theta), -2.0L * p / rot_dim);
         if (scaling == B200Q_ROPE_LINEAR) {
             f /= factor;
         } else if (scaling == B200Q_ROPE_LLAMA3) {
-            const double n = original_context * f / two_pi;  // turns over the original context
+            const long double n = original_context * f / two_pi;  // turns over the original context
             if (n < low) {
                 f /= factor;
             } else if (n <= high) {
-                const double t = (n - low) / (high - low);
-                f = (1.0 - t) * f / factor + t * f;
+                const long double t = (n - low) / (static_cast<long double>(high) - low);
+                f = (1.0L - t) * f / factor + t * f;
             }
         } else if (scaling == B200Q_ROPE_YARN) {
-            const double t = std::min(1.0, std::max(0.0, (p - y_lo) / (y_hi - y_lo)));
-            f = f / factor * t + f * (1.0 - t);
+            const long double t = std::min(1.0L, std::max(0.0L, (p - y_lo) / (static_cast<long double>(y_hi) - y_lo)));
+            f = f / factor * t + f * (1.0L - t);
         }
-        turns[p] = static_cast<unsigned long long>(std::ldexp(static_cast<long double>(f) / two_pi, 64) + 0.5L);
+        turns[p] = static_cast<unsigned long long>(std::ldexp(f / two_pi, 64) + 0.5L);
     }
     *mag = scaling == B200Q_ROPE_YARN ? 0.1 * std::log(factor) + 1.0 : 1.0;
     return B200Q_OK;
