@@ -89,19 +89,6 @@ __device__ __forceinline__ float2 lds_f2(uint32_t a) {
     asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a));
     return v;
 }
-__device__ __forceinline__ uint32_t pack2(float x, float y) {
-    const __half2 h = __floats2half2_rn(x, y);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ float2 unpack2(uint32_t h) { return __half22float2(*reinterpret_cast<const __half2*>(&h)); }
-
-// Codes + 128 (bytes of w ^ 0x80808080) as fp16 pairs: 0x64 above a byte u
-// is 1024 + u exactly; less 1152 the code.
-__device__ __forceinline__ uint32_t codes_fp16(uint32_t bytes, uint32_t sel) {
-    const uint32_t h = __byte_perm(bytes, 0x64646464u, sel);
-    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&h), __half2half2(__ushort_as_half(0x6480)));
-    return *reinterpret_cast<const uint32_t*>(&r);
-}
 
 __device__ __forceinline__ bool not_finite16(uint32_t h) {
     return (h & 0x7C00u) == 0x7C00u || (h & 0x7C000000u) == 0x7C000000u;

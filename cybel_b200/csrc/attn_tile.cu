@@ -186,11 +186,6 @@ __host__ __device__ constexpr uint32_t idesc_of(int n, bool b_mn) {
 __device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
-__device__ __forceinline__ uint32_t pack2(float x, float y) {
-    const __half2 h = __floats2half2_rn(x, y);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ float2 unpack2(uint32_t h) { return __half22float2(*reinterpret_cast<const __half2*>(&h)); }
 
 // The n lowest bits.
 __device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : (n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u); }
@@ -211,13 +206,6 @@ __device__ __forceinline__ void put2(float* p, float2 v) { p[0] = v.x, p[1] = v.
 template <int HALF>
 __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
     return (c >> 3) * HALF + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-}
-
-// Two codes + 128 as fp16: 0x64 above a byte u is 1024 + u; less 1152 the code.
-__device__ __forceinline__ uint32_t codes_fp16(uint32_t bytes, uint32_t sel) {
-    const uint32_t h = __byte_perm(bytes, 0x64646464u, sel);
-    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&h), __half2half2(__ushort_as_half(0x6480)));
-    return *reinterpret_cast<const uint32_t*>(&r);
 }
 
 // The fp16 halves of w that are not finite set to 0.
