@@ -24,8 +24,8 @@
 //
 // Q8 rows enter as their integer codes, exact in fp16; a key's scale
 // multiplies its score, a value's scale its softmax weight, relative to a
-// power of two E above the scales so far, so that the weight in fp16 neither
-// over- nor underflows. Weights are kept 2^10 above 1 for the same reason.
+// power of two E above the scales that its row has seen so far, so that the
+// weight in fp16 neither over- nor underflows. Weights are kept 2^10 above 1 for the same reason.
 #include <algorithm>
 #include <mutex>
 #include <type_traits>
@@ -209,7 +209,11 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) b200q_attn_few_kernel
     float m[NR], l[NR];
 #pragma unroll
     for (int i = 0; i < NR; ++i) m[i] = -INFINITY, l[i] = 0.0f;
-    float E = 0.0f, inv_E = 0.0f;  // Q8: the power of two that o is in units of
+    // Q8: the power of two that a row's o is in units of, above the scales that the
+    // row has seen in this warp's tiles; the warp's least.
+    float E[NR], least = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NR; ++i) E[i] = 0.0f;
 
     const TileList<kTile> tiles(s, p_lo, p_hi);
     const int stride = kWarps * static_cast<int>(C);
@@ -370,24 +374,46 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) b200q_attn_few_kernel
             top[i2] = fmaxf(top[i2], __shfl_xor_sync(0xffffffffu, top[i2], 2));
             rise |= top[i2] > m[i2] + kRise;
         }
-        float unit = 1.0f;  // Q8: change of o's unit
+        float unit[NR];  // Q8: change of o's unit
+#pragma unroll
+        for (int i2 = 0; i2 < NR; ++i2) unit[i2] = 1.0f;
         float vs[NX];
         if constexpr (Q8) {
             const float mine = fabsf(__uint_as_float(lds32(st + 2 * kTile * F::RB + (kTile + lane) * 4)));
             const float mx = mine < INFINITY ? mine : 0.0f;
-            if (__any_sync(0xffffffffu, mx >= E)) {
-                const float e2 = pow2_above(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx))));
-                unit = E / e2;  // both powers of two (0 at the first tile, where o is 0)
-                E = e2;
-                inv_E = 1.0f / E;
-            }
 #pragma unroll
             for (int nb = 0; nb < NK; ++nb) {
                 const float2 v2 = lds_f2(st + 2 * kTile * F::RB + (kTile + 8 * nb + 2 * c) * 4);
-                vs[2 * nb] = v2.x * inv_E, vs[2 * nb + 1] = v2.y * inv_E;
+                vs[2 * nb] = v2.x, vs[2 * nb + 1] = v2.y;
+            }
+            if (__any_sync(0xffffffffu, mx >= least)) {
+                const float all = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx)));
+                least = INFINITY;
+#pragma unroll
+                for (int i2 = 0; i2 < NR; ++i2) {
+                    float most = all;
+                    if (!whole) {  // of the positions that the row sees: others' would push its weights below fp16
+                        most = 0.0f;
+#pragma unroll
+                        for (int v = 0; v < NX; ++v) {
+                            const float y = x[i2][v] == -INFINITY ? 0.0f : fabsf(vs[v]);
+                            most = y < INFINITY ? fmaxf(most, y) : most;
+                        }
+                        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+                    }
+                    if (most >= E[i2]) {
+                        const float e2 = fminf(pow2_above(most), 8.5070591730e37f);  // 2^126
+                        unit[i2] = E[i2] / e2;  // both powers of two (0 at the first tile, where o is 0)
+                        E[i2] = e2;
+                        rise = true;
+                    }
+                    least = fminf(least, E[i2]);
+                }
+                least = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(least)));
             }
         }
-        if (__any_sync(0xffffffffu, rise) || unit != 1.0f) {
+        if (__any_sync(0xffffffffu, rise)) {
 #pragma unroll
             for (int i2 = 0; i2 < NR; ++i2) {
                 const float mn = top[i2] > m[i2] + kRise ? top[i2] : m[i2];
@@ -398,10 +424,10 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) b200q_attn_few_kernel
                 for (int n = 0; n < NB; ++n) {
                     if constexpr (SPLIT) {
 #pragma unroll
-                        for (int v = 0; v < 4; ++v) o[n][v] *= f * unit;
+                        for (int v = 0; v < 4; ++v) o[n][v] *= f * unit[i2];
                     } else {
-                        o[n][2 * i2] *= f * unit;
-                        o[n][2 * i2 + 1] *= f * unit;
+                        o[n][2 * i2] *= f * unit[i2];
+                        o[n][2 * i2 + 1] *= f * unit[i2];
                     }
                 }
             }
@@ -411,6 +437,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) b200q_attn_few_kernel
 #pragma unroll
         for (int i2 = 0; i2 < NR; ++i2) {
             const float base = m[i2] == -INFINITY ? 0.0f : kLift - m[i2];
+            const float inv_E = __int_as_float(0x7F000000 - __float_as_int(E[i2]));  // (of a power of two, 2^126 at most)
 #pragma unroll
             for (int f = 0; f < kTile / 16; ++f) {
                 float p[4];
@@ -418,7 +445,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) b200q_attn_few_kernel
                 for (int v = 0; v < 4; ++v) {
                     p[v] = ex2(x[i2][4 * f + v] + base);
                     l[i2] += p[v];
-                    if constexpr (Q8) p[v] = x[i2][4 * f + v] == -INFINITY ? 0.0f : p[v] * vs[4 * f + v];
+                    if constexpr (Q8) p[v] = x[i2][4 * f + v] == -INFINITY ? 0.0f : p[v] * (vs[4 * f + v] * inv_E);
                 }
                 if constexpr (SPLIT) {
                     pa[f][0] = pack2(p[0], p[1]);
@@ -521,7 +548,6 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) b200q_attn_few_kernel
 
     // ---- join the warps of the CTA, then the CTAs of the cluster
     float* part = reinterpret_cast<float*>(smem + warp * F::kWarpBytes);  // [R][D]
-    const float out_unit = Q8 ? E : 1.0f;
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
@@ -536,7 +562,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) b200q_attn_few_kernel
                 // (the low parts of weights turn an infinite value into NaN: leave them out then)
                 const float val = !SPLIT ? o[n][2 * i + v]
                                         : o[n][v] + (fabsf(o[n][2 + v]) < INFINITY ? o[n][2 + v] : 0.0f);
-                part[(g + 8 * i) * D + e] = val * out_unit;
+                part[(g + 8 * i) * D + e] = Q8 ? val * E[i] : val;
             }
         }
     }

@@ -20,8 +20,8 @@
 //    clocks a step, issuing one tile's while the other's were due).
 //
 // Q8 codes enter the products as they are; their scales multiply scores and
-// weights in fp32, the latter relative to a power of two above the scales so
-// far. (Code x scale rounded to fp16 for the products took 176 us instead of
+// weights in fp32, the latter relative to a power of two above the scales that
+// the row has seen so far. (Code x scale rounded to fp16 for the products took 176 us instead of
 // 208 at 4096 tokens, 32/8 heads, but each of the two roundings was as large as
 // the output's own, and the error against 64 bits 2.4 times as large instead of
 // 1.4 times. The weights' rounding to fp16 makes the rest of that factor.)
@@ -699,7 +699,7 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
         const Steps mine(sight, list, i0, job.lo[t], job.hi[t]);
         const int t_lo = job.lo[t], t_hi = job.hi[t];
         float m = -INFINITY, l = 0.0f;
-        float E = 0.0f, log_E = 0.0f;  // SC: weights, their sum and the output are relative to E
+        float E = 0.0f, log_E = 0.0f;  // SC: the row's weights, their sum and its output are relative to E
         // PREC: 64 columns of the output, o keep + the product at f (o 0 before `add`).
         auto take = [&](uint32_t f, uint32_t o_at, bool add, float keep) {
 #pragma unroll
@@ -756,12 +756,26 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
             float unit = 1.0f;
             if constexpr (SC) {
                 const float4 vm = *reinterpret_cast<const float4*>(md.vmax);
-                const float mx = fmaxf(fmaxf(vm.x, vm.y), fmaxf(vm.z, vm.w));
+                float mx = fmaxf(fmaxf(vm.x, vm.y), fmaxf(vm.z, vm.w));
                 if (mx >= E) {
-                    const float e2 = fmaxf(pow2_above(mx), 8.6736173799e-19f);  // 2^-60
-                    unit = E / e2;  // powers of two; 0 at the first step
-                    E = e2;
-                    log_E = static_cast<float>((__float_as_int(E) >> 23) - 127);
+                    if (!whole) {  // of the positions that the row sees: others' would push its weights below fp16
+                        const uint32_t at = smem_addr(md.vs);
+                        mx = 0.0f;
+#pragma unroll
+                        for (int c = 0; c < kRows; c += 4) {
+                            const float4 v = lds_f4(at + c * 4);
+                            const float f[4] = {fabsf(v.x), fabsf(v.y), fabsf(v.z), fabsf(v.w)};
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                if ((see[c >> 5] & (1u << ((c + k) & 31))) && f[k] < INFINITY) mx = fmaxf(mx, f[k]);
+                        }
+                    }
+                    if (mx >= E) {
+                        const float e2 = fmaxf(pow2_above(mx), 8.6736173799e-19f);  // 2^-60
+                        unit = E / e2;  // powers of two; 0 at the first step
+                        E = e2;
+                        log_E = static_cast<float>((__float_as_int(E) >> 23) - 127);
+                    }
                 }
             }
             ok = __all_sync(0xffffffffu, wait(sready(t), steps & 1));

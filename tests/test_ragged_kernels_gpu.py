@@ -224,3 +224,34 @@ def test_pools_past_32_bits(dtype, q8):
     assert np.abs(got - first).max() <= np.abs(first).max() * (0.51 / 127 if q8 else 2.0 ** -11)
     low = c.k[:slots - 4]
     assert not any(bool(low[a:a + 100].any()) for a in range(0, slots - 4, 100))  # nothing fell elsewhere
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "fp16"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("lens", [FEW, MANY])
+@pytest.mark.parametrize("form", ["causal", "window", "prefix"])
+def test_large_value_scales_matter_to_rows_that_see_them_alone(form, lens, hd, dtype):
+    """Q8 value scales 2^30 times the others' (fp16 rows: 2^18, to stay in
+    their range) at positions that a part of the rows sees: the others lose
+    nothing (the unit that a row's weights are kept in follows the scales that
+    the row sees)."""
+    import torch
+
+    c, batch, g = _cache(lens, 2, hd, 16, True, seed=hd)
+    q = _randn(batch, 8, hd, dtype, g)
+    assert _reaches(lens, q, batch, 2, window=60 if form == "window" else 0, prefix=form == "prefix", q8=True)
+    kw, ref = {}, {}
+    if dtype == "fp16":
+        c.vs *= 2.0 ** -10
+    if form == "window":
+        kw["window"] = ref["window"] = 60
+    if form == "prefix":
+        p = [n - m // 2 if m > 1 else n // 2 for m, n in zip(*lens)]
+        kw["prefix"], ref["prefix"] = torch.tensor(p, dtype=torch.int32, device="cuda"), p
+    for b, (m, n) in enumerate(zip(*lens)):
+        for j in range(n - (m // 3 if m > 20 else 1), n) if form != "window" else range(n - m - 1, n - m + 1):
+            if j >= 0:
+                c.vs[c.table_host[0, b, j // 16], :, j % 16] *= 2.0 ** (30 if dtype == "fp32" else 18)
+    out = c.attend(0, q, batch, **kw)
+    _clean()
+    _check(c, 0, batch, q, out, **ref)

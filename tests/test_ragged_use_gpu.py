@@ -188,7 +188,8 @@ def _check(c, layer, batch, q, got, scale=None, cap=0.0, slopes=None, window=0, 
             extra = torch.where(odd[a, jj], v[a, jj], torch.zeros_like(v[a, jj]))
             want[a] += torch.where((p[a, :, :, jj] > 0)[..., None], extra, torch.zeros_like(extra))
         tol = bound + spread * (2.0 ** -10 + 2.0 ** -14 if f16 else 2.0 ** -19) + (2.0 ** -24 if f16 else 1e-30)
-        tol = tol + n * 2.0 ** -34 * fine.abs().max()
+        most = fine.abs().amax(-1)[:, None, None, :].masked_fill(~see, 0.0).amax(-1, keepdim=True)  # of what the row sees
+        tol = tol + n * 2.0 ** -34 * most
         flat = (lambda t: t.permute(2, 0, 1, 3).reshape(m, heads, hd))
         want, tol = flat(want), flat(tol)
         mine = got[at:at + m].double()
