@@ -333,9 +333,10 @@ __device__ __forceinline__ float q8_scale(float amax) {
     return amax > 0.0f ? __fdiv_rn(amax, 127.0f) : __fdiv_rn(1.0f, 127.0f);
 }
 // round() of the definition (halves away from zero), as a byte: to the nearest
-// integer by adding 1.5 2^23, halves that went to the even side put right.
+// integer by adding 1.5 2^23, halves that went to the even side put right. NaN
+// (also an infinity over its scale) is 0, as the conversion to an integer makes it.
 __device__ __forceinline__ uint32_t q8_code(float x, float inv) {
-    const float y = fminf(fmaxf(__fmul_rn(x, inv), -127.0f), 127.0f);
+    const float p = __fmul_rn(x, inv), y = p == p ? fminf(fmaxf(p, -127.0f), 127.0f) : 0.0f;
     const float t = __fadd_rn(y, 12582912.0f);
     const float rest = __fsub_rn(y, __fsub_rn(t, 12582912.0f));  // exact
     int c = __float_as_int(t);

@@ -318,3 +318,45 @@ def test_a_window_past_every_length_is_none(lens, window):
     assert lens is FEW or _both(q, batch, 2)
     assert torch.equal(c.attend(0, q, batch, window=window), c.attend(0, q, batch))
     _clean()
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "fp16"])
+def test_q8_rows_are_those_of_the_one_position_attention(dtype):
+    """The codes and scales that append stores are those that
+    PagedKVCache.attention stores for the same rows, whatever the rows hold:
+    NaN, infinities, numbers too small for a scale, halves between two codes."""
+    import torch
+
+    from cybel_b200.kv_cache import PagedKVCache
+    from cybel_b200.paged_attention import RaggedBatch, RopeTable
+
+    seqs, kv = 9, 2
+    g = torch.Generator(device="cuda")
+    g.manual_seed(6)
+    k, v = (torch.randn(seqs, kv, 128, generator=g, device="cuda") for _ in range(2))
+    for t in (k, v):
+        t[1, 0, 5] = float("nan")
+        t[2, 1, 7] = float("inf")
+        t[3, 0, 9] = float("-inf")
+        t[3, 0, 11] = float("nan")
+        t[4] = float("nan")
+        t[5] = 0.0
+        t[6] = 0.0
+        t[6, :, ::3] = 2.0 ** -149 if dtype == "fp32" else 2.0 ** -24
+        t[7] = (torch.randint(-254, 255, t[7].shape, generator=g, device="cuda") / 2).float()
+        t[7, :, 0] = 127.0  # scale 1: halves
+    if dtype == "fp16":
+        k, v = k.half(), v.half()
+    caches = [PagedKVCache(1, kv, 16, batch=seqs, page_size=16, q8=True) for _ in range(2)]
+    for c in caches:
+        c.ensure(0)
+    caches[0].append(0, k, v, RaggedBatch([1] * seqs, [1] * seqs), rope=RopeTable(128))
+    q, out = torch.ones(seqs, kv, 128, device="cuda"), torch.empty(seqs, kv, 128, device="cuda")
+    kf, vf = k.float(), v.float()
+    caches[1].attention(0, q.data_ptr(), kf.data_ptr(), vf.data_ptr(), 0, kv, 10000.0, out.data_ptr(), None, 0,
+                        torch.cuda.current_stream().cuda_stream)
+    _clean()
+    for b in range(seqs):
+        for h in range(kv):
+            for got, want in zip(caches[0].rows(0, b, h, 0, 1), caches[1].rows(0, b, h, 0, 1)):
+                assert np.array_equal(got, want), (b, h, got, want)
