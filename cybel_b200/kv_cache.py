@@ -111,6 +111,8 @@ class PagedKVCache:
             raise ValueError("k and v must be fp16 [layers][kv_heads][max_ctx][head_dim]")
         if not (k.is_contiguous() and v.is_contiguous()) or k.shape[3] not in HEAD_DIMS:
             raise ValueError("k and v must be contiguous, heads of 64 or 128")
+        if k.device != v.device or not k.numel():
+            raise ValueError("k and v must be on one device and hold a position")
         self = cls.__new__(cls)
         self.layers, self.kv_heads, self.max_seq, self.head_dim = k.shape
         self.batch, self.pages_per_seq, self.page_size, self.q8 = 1, 1, self.max_seq, False
@@ -278,8 +280,10 @@ class PagedKVCache:
         slopes[h] * distance (fp32 [heads]) when slopes are given; causal,
         within the last `window` positions when window > 0, plus the first
         prefix[b] positions (int32 [sequences]) for every row. q [n_tokens]
-        [heads][head_dim] fp32 or fp16; returns ``out`` (or a new tensor) of
-        q's type and shape. Current stream; b200q_attention_paged."""
+        [heads][head_dim] fp32 or fp16, rows 16-byte aligned; returns ``out``
+        (may be q; or a new tensor) of q's type and shape, whose rows behind
+        the last sequence are left as they are (a new tensor's: undefined).
+        Current stream; b200q_attention_paged."""
         from .paged_attention import attend
 
         return attend(self, layer, q, batch, out, scale, softcap, slopes, window, prefix)

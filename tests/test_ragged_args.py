@@ -54,3 +54,11 @@ def test_rope_context_past_32_bits_is_refused():
         RopeTable(128, scaling="llama3", factor=8.0, original_context=2 ** 32 + 8192, device="cpu")
     with pytest.raises((ValueError, _native.NativeError)):
         RopeTable(2 ** 32 + 128, device="cpu")
+
+
+def test_a_view_of_caches_on_two_devices_is_refused():
+    k = torch.zeros(1, 2, 16, 64, dtype=torch.float16)
+    with pytest.raises(ValueError):
+        PagedKVCache.over_contiguous(k, torch.zeros_like(k, device="meta"))
+    with pytest.raises(ValueError):  # no position to hold
+        PagedKVCache.over_contiguous(k[:, :, :0], k[:, :, :0])
