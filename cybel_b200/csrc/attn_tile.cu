@@ -837,11 +837,14 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
                 }
                 if (a.slopes) {
                     const float d0 = static_cast<float>(pos - j0);
-                    if (j0 + kRows - 1 <= t_lo) {  // all behind the rows: the distance is d0 - c
-                        row_off = -slope * d0;
+                    if (j0 + kRows - 1 <= t_lo) {
+                        // All behind the rows: the distance of the step's last position and the rest,
+                        // so that the nearest biases, which matter most, are the smallest numbers.
+                        constexpr int kEnd = kRows - 1;
+                        row_off = -slope * (d0 - kEnd);
 #pragma unroll
                         for (int c = 0; c < kRows; c += 2)
-                            put2(x + c, fma2(both(slope), make_float2(c, c + 1), make_float2(x[c], x[c + 1])));
+                            put2(x + c, fma2(both(slope), make_float2(c - kEnd, c + 1 - kEnd), make_float2(x[c], x[c + 1])));
                     } else {
 #pragma unroll
                         for (int c = 0; c < kRows; ++c) x[c] = fmaf(-slope, fabsf(d0 - static_cast<float>(c)), x[c]);

@@ -255,3 +255,23 @@ def test_large_value_scales_matter_to_rows_that_see_them_alone(form, lens, hd, d
     out = c.attend(0, q, batch, **kw)
     _clean()
     _check(c, 0, batch, q, out, **ref)
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("hd,heads,kv", [(128, 8, 2), (64, 33, 1)])
+@pytest.mark.parametrize("lens", [FEW, MANY])
+def test_steep_distance_biases_keep_the_near_positions_exact(lens, hd, heads, kv, q8):
+    """Slopes near 1, with which the nearest positions have nearly all the
+    weight: a bias is rounded by its own size, not by that of the farthest
+    position of its step. (One-hot queries of small scores: no other error.)"""
+    import torch
+
+    from tests.test_ragged_use_gpu import _one_hot
+
+    c, batch, g = _cache(lens, kv, hd, 48, q8, seed=heads)
+    q = _one_hot(batch.n_tokens, heads, hd, 0.015625, g)
+    assert _reaches(lens, q, batch, kv, q8=q8)
+    slopes = torch.tensor([0.97 - 0.015 * h for h in range(heads)], device="cuda")
+    out = c.attend(0, q, batch, scale=1.0, slopes=slopes)
+    _clean()
+    _check(c, 0, batch, q, out, scale=1.0, slopes=slopes, terms=1)
