@@ -576,6 +576,14 @@ int widest(size_t es, std::initializer_list<const void*> ptrs, std::initializer_
 
 size_t elem_size(int dtype) { return dtype == B200Q_F32 ? 4 : 2; }
 
+const long double kTwoPi = 6.283185307179586476925286766559L;
+
+// The pair whose frequency makes `turns` turns over `context` positions.
+double pair_of_turns(double turns, int context, int rot_dim, double theta) {
+    return static_cast<double>(rot_dim * std::log(context / (turns * kTwoPi)) /
+                               (2.0L * std::log(static_cast<long double>(theta))));
+}
+
 }  // namespace
 
 int rope_table(int rot_dim, double theta, int scaling, double factor, double low, double high, int original_context,
@@ -586,16 +594,10 @@ int rope_table(int rot_dim, double theta, int scaling, double factor, double low
     if (scaling != B200Q_ROPE_PLAIN && !(factor >= 1.0 && std::isfinite(factor))) return B200Q_EINVAL;
     const bool bands = scaling == B200Q_ROPE_LLAMA3 || scaling == B200Q_ROPE_YARN;
     if (bands && (original_context <= 0 || !(low > 0.0) || !(high > low) || !std::isfinite(high))) return B200Q_EINVAL;
-    const long double two_pi = 6.283185307179586476925286766559L;
     double y_lo = 0.0, y_hi = 1.0;
     if (scaling == B200Q_ROPE_YARN) {
-        // the pair whose frequency makes beta turns over the original context
-        auto at = [&](double beta) {
-            return static_cast<double>(rot_dim * std::log(original_context / (beta * two_pi)) /
-                                       (2.0L * std::log(static_cast<long double>(theta))));
-        };
-        y_lo = std::max(0.0, std::floor(at(high)));
-        y_hi = std::min(rot_dim - 1.0, std::ceil(at(low)));
+        y_lo = std::max(0.0, std::floor(pair_of_turns(high, original_context, rot_dim, theta)));
+        y_hi = std::min(rot_dim - 1.0, std::ceil(pair_of_turns(low, original_context, rot_dim, theta)));
         if (!(y_hi > y_lo)) y_hi = y_lo + 0.001;
     }
     for (int p = 0; p < rot_dim / 2; ++p) {
@@ -603,7 +605,7 @@ int rope_table(int rot_dim, double theta, int scaling, double factor, double low
         if (scaling == B200Q_ROPE_LINEAR) {
             f /= factor;
         } else if (scaling == B200Q_ROPE_LLAMA3) {
-            const long double n = original_context * f / two_pi;  // turns over the original context
+            const long double n = original_context * f / kTwoPi;  // turns over the original context
             if (n < low) {
                 f /= factor;
             } else if (n <= high) {
@@ -611,10 +613,11 @@ int rope_table(int rot_dim, double theta, int scaling, double factor, double low
                 f = (1.0L - t) * f / factor + t * f;
             }
         } else if (scaling == B200Q_ROPE_YARN) {
-            const long double t = std::min(1.0L, std::max(0.0L, (p - y_lo) / (static_cast<long double>(y_hi) - y_lo)));
+            const long double at_p = (p - y_lo) / (static_cast<long double>(y_hi) - y_lo);
+            const long double t = at_p < 0.0L ? 0.0L : at_p > 1.0L ? 1.0L : at_p;
             f = f / factor * t + f * (1.0L - t);
         }
-        turns[p] = static_cast<unsigned long long>(std::ldexp(f / two_pi, 64) + 0.5L);
+        turns[p] = static_cast<unsigned long long>(std::ldexp(f / kTwoPi, 64) + 0.5L);
     }
     *mag = scaling == B200Q_ROPE_YARN ? 0.1 * std::log(factor) + 1.0 : 1.0;
     return B200Q_OK;
