@@ -31,7 +31,9 @@ namespace {
 // fp16 14 against 19 for 1, 29 against 25 for 4. Of 360 such batches two take
 // the kernel that is slower by more than 8 percent, by 20 at most. A prompt of
 // 600 tokens on one kv head, 4 heads, fp32: 21 against 34 us; of 128 tokens, 32/8
-// heads, fp16: 9 against 12; of 256: 17 against 14, the tile kernel's.)
+// heads, fp16: 9 against 12; of 256: 17 against 14, the tile kernel's.) All of it
+// for heads of 128 with plain scores and sequences of like lengths: heads of 64,
+// caps, biases and lengths that differ do not enter the estimate.
 int few_rows(int batch, int n_kv, long long total_rows, int most, int max_kv, bool fp32, bool q8, int sms) {
     if (most <= 32) return 32;
     const long long fu = static_cast<long long>(batch) * n_kv * ((most + (fp32 ? 7 : 15)) / (fp32 ? 8 : 16));

@@ -215,7 +215,7 @@ LENS = {
     "step": ([1, 1, 1, 0, 1], [1, 64, 129, 40, 700]),
     "few": ([3, 1, 8, 2, 0, 5], [3, 200, 333, 65, 0, 128]),
     "prompts": ([257, 1, 130, 33], [257, 300, 131, 480]),
-    "many": ([257, 1, 130, 0, 270], [257, 300, 700, 40, 900]),  # the many-row kernel's at any shape below
+    "many": ([257, 1, 130, 0, 270], [257, 300, 700, 40, 900]),  # the many-row kernel's at most shapes below
 }
 SHAPES = [(128, 4, 1), (128, 8, 2), (64, 3, 1), (128, 16, 2), (64, 10, 2), (128, 2, 2)]  # hd, heads, kv_heads
 

@@ -360,3 +360,21 @@ def test_q8_rows_are_those_of_the_one_position_attention(dtype):
         for h in range(kv):
             for got, want in zip(caches[0].rows(0, b, h, 0, 1), caches[1].rows(0, b, h, 0, 1)):
                 assert np.array_equal(got, want), (b, h, got, want)
+
+
+def test_heads_of_64_have_no_one_position_attention():
+    """A cache of 64-wide heads serves append and attend; the one-position
+    attention, built for 128, refuses it before a launch."""
+    import torch
+
+    from cybel_b200 import _native
+    from cybel_b200.kv_cache import PagedKVCache
+
+    c = PagedKVCache(1, 1, 32, batch=1, page_size=16, q8=False, head_dim=64)
+    c.ensure(0)
+    x, out = torch.ones(64, device="cuda"), torch.full((64,), 3.0, device="cuda")
+    with pytest.raises(_native.NativeError):
+        c.attention(0, x.data_ptr(), x.data_ptr(), x.data_ptr(), 0, 1, 10000.0, out.data_ptr(), None, 0,
+                    torch.cuda.current_stream().cuda_stream)
+    _clean()
+    assert (out == 3).all() and not c.k.any()
