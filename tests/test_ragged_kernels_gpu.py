@@ -275,3 +275,24 @@ def test_steep_distance_biases_keep_the_near_positions_exact(lens, hd, heads, kv
     out = c.attend(0, q, batch, scale=1.0, slopes=slopes)
     _clean()
     _check(c, 0, batch, q, out, scale=1.0, slopes=slopes, terms=1)
+
+
+@pytest.mark.parametrize("dtype,q8", TYPES)
+@pytest.mark.parametrize("lens", [FEW, MANY])
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+def test_a_query_row_that_is_not_finite_stays_alone(cap, lens, dtype, q8):
+    """NaN and infinities in a few query rows: every other row has the bits it
+    has without them."""
+    import torch
+
+    c, batch, g = _cache(lens, 2, 128, 48, q8, seed=7)
+    q = _randn(batch, 8, 128, dtype, g)
+    assert _reaches(lens, q, batch, 2, q8=q8)
+    want = c.attend(0, q, batch, softcap=cap)
+    bad = torch.zeros(batch.n_tokens, 8, dtype=torch.bool, device="cuda")
+    for i, x in ((0, float("nan")), (5, float("inf")), (8, float("-inf")), (batch.n_tokens - 3, float("nan"))):
+        q[i, i % 8, 9] = x
+        bad[i, i % 8] = True
+    out = c.attend(0, q, batch, softcap=cap)
+    _clean()
+    assert torch.equal(out[~bad], want[~bad]) and torch.isnan(out[0, 0]).all()
