@@ -39,6 +39,7 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kMaxCluster = 16;  // beyond 8 only where the device allows it
+constexpr int kPlainSum = 32768;  // positions of a warp whose sum the tensor cores keep: 2^-12.2 of it are lost
 constexpr float kRise = 4.0f;    // a row's reference maximum follows once exceeded by this (log2)
 constexpr float kLift = 10.0f;   // weights are 2^(score - maximum + kLift): at most 2^14 in fp16
 
@@ -84,6 +85,40 @@ __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uin
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// The tensor cores cut an accumulator off with each product: 0.11 x 2^-24 of a
+// sum of one sign per position. fp32 rows add the products themselves: their
+// error at 8000 positions is 3e-7 instead of 6e-6, for 1 to 3 percent of the time
+// (one row of 32/8 heads over 2048 positions 9.0 -> 9.2 us, 64 over 4000 175 -> 177;
+// Q8, the two parts joined at once, 110 -> 112; apart they spilled: 133).
+// fp16 rows (5 percent) take it, up to kPlainSum positions a warp.
+__device__ __forceinline__ void add4(float (&d)[4], const float (&t)[4]) {
+    const float2 x = add2(make_float2(d[0], d[1]), make_float2(t[0], t[1]));
+    const float2 y = add2(make_float2(d[2], d[3]), make_float2(t[2], t[3]));
+    d[0] = x.x, d[1] = x.y, d[2] = y.x, d[3] = y.y;
+}
+// The product's two parts (rows g and g + 8) added to d's first two.
+__device__ __forceinline__ void add_parts(float (&d)[4], const float (&t)[4]) {
+    const float2 p = add2(make_float2(t[0], t[1]), make_float2(t[2], t[3]));
+    const float2 x = add2(make_float2(d[0], d[1]), p);
+    d[0] = x.x, d[1] = x.y;
+}
+// d plus the product. OWN: the product gets an accumulator of its own and is
+// added to d in fp32; else the tensor core adds it, and cuts the sum off.
+template <bool OWN>
+__device__ __forceinline__ void mma_onto(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (OWN) {
+        float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        mma16(t, a, b0, b1);
+        add4(d, t);
+    } else {
+        mma16(d, a, b0, b1);
+    }
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+    return v;
+}
 __device__ __forceinline__ float2 lds_f2(uint32_t a) {
     float2 v;
     asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a));
@@ -117,6 +152,9 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) b200q_attn_few_kernel
     constexpr int R = F::R, KS = D / 16, NB = D / 8, NS = F::NS, kTile = F::kTile;
     constexpr int NK = kTile / 8;  // blocks of 8 positions
     constexpr uint32_t kAll = kTile == 32 ? 0xFFFFFFFFu : 0xFFFFu;
+    // o holds the sum of the two parts (in o[.][0] and o[.][1]) where products are
+    // added to it in fp32 and no value is infinite by itself, but by its scale.
+    constexpr bool kJoined = Q8 && FP32;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint32_t present[kWarps][8];  // per stage: which of its positions have a row
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
@@ -424,7 +462,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) b200q_attn_few_kernel
                 for (int n = 0; n < NB; ++n) {
                     if constexpr (SPLIT) {
 #pragma unroll
-                        for (int v = 0; v < 4; ++v) o[n][v] *= f * unit[i2];
+                        for (int v = 0; v < (kJoined ? 2 : 4); ++v) o[n][v] *= f * unit[i2];
                     } else {
                         o[n][2 * i2] *= f * unit[i2];
                         o[n][2 * i2 + 1] *= f * unit[i2];
@@ -451,8 +489,13 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) b200q_attn_few_kernel
                     pa[f][0] = pack2(p[0], p[1]);
                     pa[f][2] = pack2(p[2], p[3]);
                     const float2 h0 = unpack2(pa[f][0]), h1 = unpack2(pa[f][2]);
-                    pa[f][1] = pack2(p[0] - h0.x, p[1] - h0.y);
-                    pa[f][3] = pack2(p[2] - h1.x, p[3] - h1.y);
+                    float low[4] = {p[0] - h0.x, p[1] - h0.y, p[2] - h1.x, p[3] - h1.y};
+                    if constexpr (kJoined) {  // an infinity is the upper part's alone
+#pragma unroll
+                        for (int v = 0; v < 4; ++v) low[v] = fabsf(p[v]) < INFINITY ? low[v] : 0.0f;
+                    }
+                    pa[f][1] = pack2(low[0], low[1]);
+                    pa[f][3] = pack2(low[2], low[3]);
                 } else {
                     pa[f][i2] = pack2(p[0], p[1]);
                     pa[f][2 + i2] = pack2(p[2], p[3]);
@@ -499,6 +542,41 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) b200q_attn_few_kernel
             }
         }
         // ---- O += P V
+        if constexpr (kJoined) {
+            // As below, but two words of the values at a time, so that both fragments'
+            // products share an accumulator.
+            constexpr int NF = kTile / 16;
+#pragma unroll
+            for (int h = 0; h < D / 64; ++h) {
+                uint32_t wv[NF][4][2];
+#pragma unroll
+                for (int f = 0; f < NF; ++f)
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) {
+                        const int r = 2 * c + (t & 1) + 8 * (t >> 1);
+                        const uint2 w = lds64(vt + (f * 16 + r) * F::RB + (D == 128 ? v_chunk<D, Q8>(r, g) * 16 + h * 8
+                                                                                   : v_chunk<D, Q8>(r, g >> 1) * 16 + (g & 1) * 8));
+                        wv[f][t][0] = w.x ^ 0x80808080u, wv[f][t][1] = w.y ^ 0x80808080u;
+                    }
+#pragma unroll
+                for (int w = 0; w < 2; ++w)
+#pragma unroll
+                    for (int hf = 0; hf < 2; ++hf) {
+                        const uint32_t sel = hf ? 0x7362u : 0x5140u;
+                        float s0[4] = {0.0f, 0.0f, 0.0f, 0.0f}, s1[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                        for (int f = 0; f < NF; ++f) {
+                            const uint32_t b0 = __byte_perm(wv[f][0][w], wv[f][1][w], sel);
+                            const uint32_t b1 = __byte_perm(wv[f][2][w], wv[f][3][w], sel);
+                            mma16(s0, pa[f], codes_fp16(b0, 0x4140), codes_fp16(b1, 0x4140));
+                            mma16(s1, pa[f], codes_fp16(b0, 0x4342), codes_fp16(b1, 0x4342));
+                        }
+                        add_parts(o[4 * (2 * h + w) + 2 * hf], s0);
+                        add_parts(o[4 * (2 * h + w) + 2 * hf + 1], s1);
+                    }
+            }
+            continue;
+        }
 #pragma unroll
         for (int f = 0; f < kTile / 16; ++f) {
             const uint32_t vf = vt + f * 16 * F::RB;
@@ -508,8 +586,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) b200q_attn_few_kernel
                     uint32_t v4[4];
                     const int r = (lane & 7) + 8 * ((lane >> 3) & 1);
                     ldsm4t(v4, vf + r * F::RB + v_chunk<D, Q8>(r, n + (lane >> 4)) * 16);
-                    mma16(o[n], pa[f], v4[0], v4[1]);
-                    mma16(o[n + 1], pa[f], v4[2], v4[3]);
+                    mma_onto<FP32>(o[n], pa[f], v4[0], v4[1]);
+                    mma_onto<FP32>(o[n + 1], pa[f], v4[2], v4[3]);
                 }
             } else {
                 // Block n, column g: element g * NB + n, so that a lane's elements of
@@ -560,8 +638,9 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) b200q_attn_few_kernel
                 const int col = 2 * c + v;
                 const int e = Q8 ? col * NB + n : n * 8 + col;
                 // (the low parts of weights turn an infinite value into NaN: leave them out then)
-                const float val = !SPLIT ? o[n][2 * i + v]
-                                        : o[n][v] + (fabsf(o[n][2 + v]) < INFINITY ? o[n][2 + v] : 0.0f);
+                const float val = !SPLIT    ? o[n][2 * i + v]
+                                  : kJoined ? o[n][v]
+                                            : o[n][v] + (fabsf(o[n][2 + v]) < INFINITY ? o[n][2 + v] : 0.0f);
                 part[(g + 8 * i) * D + e] = Q8 ? val * E[i] : val;
             }
         }
@@ -690,11 +769,13 @@ int few_block_rows(bool fp32, int max_rows) { return fp32 || max_rows <= 8 ? 8 :
 // the halves), and about 64 positions a warp. Measured at 4 x 8 rows of 2000
 // positions: 17 us for one wave, 24 for two; 64 sequences of 100-8000: 191, 175,
 // 186 us for 1, 2, 4. More than 8 only up to three quarters of a wave: larger
-// clusters do not fill the GPCs (24 of 16 took 36 us at 8000 positions, of 13 23).
+// clusters do not fill the GPCs (24 of 16 took 36 us at 8000 positions, of 13 23),
+// or for sums of more than kPlainSum positions a warp.
 int few_split(long long units, int max_kv, int sms) {
     const long long slots = few_slots(sms);
     long long c = std::max<long long>(slots / units, 2);
     if (c > 8) c = std::max<long long>(8, std::min<long long>(kMaxCluster, slots * 3 / 4 / units));
+    c = std::max(c, std::min<long long>(kMaxCluster, (max_kv + kWarps * kPlainSum - 1ll) / (kWarps * kPlainSum)));
     return static_cast<int>(std::max<long long>(1, std::min<long long>(c, (max_kv + kWarps * 64 - 1) / (kWarps * 64))));
 }
 

@@ -8,7 +8,7 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
-from tests.test_ragged_use_gpu import FEW, MANY, _both, _cache, _check, _clean, _plan
+from tests.test_ragged_use_gpu import FEW, MANY, _both, _cache, _check, _clean, _one_hot, _plan
 
 pytestmark = pytest.mark.gpu
 
@@ -266,8 +266,6 @@ def test_steep_distance_biases_keep_the_near_positions_exact(lens, hd, heads, kv
     position of its step. (One-hot queries of small scores: no other error.)"""
     import torch
 
-    from tests.test_ragged_use_gpu import _one_hot
-
     c, batch, g = _cache(lens, kv, hd, 48, q8, seed=heads)
     q = _one_hot(batch.n_tokens, heads, hd, 0.015625, g)
     assert _reaches(lens, q, batch, kv, q8=q8)
@@ -296,3 +294,59 @@ def test_a_query_row_that_is_not_finite_stays_alone(cap, lens, dtype, q8):
     out = c.attend(0, q, batch, softcap=cap)
     _clean()
     assert torch.equal(out[~bad], want[~bad]) and torch.isnan(out[0, 0]).all()
+
+
+@pytest.mark.parametrize("dtype,q8", TYPES)
+@pytest.mark.parametrize("seqs,m,n", [(64, 1, 8000), (64, 1, 32000), (16, 8, 30000), (2, 600, 6000), (1, 1300, 30000)])
+def test_long_sums_of_one_sign(seqs, m, n, dtype, q8):
+    """Values that are all near 1, whose sums grow with every position: what a
+    sum loses must not grow with its length. (The tensor cores cut their
+    accumulators off, by 0.11 x 2^-24 a position. One-hot queries, whose scores
+    carry no error of a sum that would cover it.)"""
+    heads = 8 if m < 600 else 32
+    kv = 8 if m < 600 else 1
+    c, batch, g = _cache(([m] * seqs, [n] * seqs), kv, 128, 256, q8, seed=1)
+    if q8:
+        c.v.random_(90, 128)
+        c.vs.fill_(0.01)
+    else:
+        c.v.normal_(1.0, 0.1)
+    q = _one_hot(batch.n_tokens, heads, 128, 0.0625, g).to(_dt(dtype))
+    assert bool(_plan(q, batch, kv, q8=q8)[2]) == (m >= 600)
+    out = c.attend(0, q, batch, scale=1.0)
+    _clean()
+    rows = list(range(0, m, max(m // 3, 1)))  # some rows of the first sequence
+    from cybel_b200.paged_attention import RaggedBatch
+
+    for t in rows:
+        one = RaggedBatch([1], [n - m + t + 1])
+        _check(c, 0, one, q[t:t + 1], out[t:t + 1], scale=1.0, terms=1)
+
+
+@pytest.mark.parametrize("q8", [False, True])
+def test_a_step_over_two_million_positions(q8):
+    """fp16 rows of many sequences at once (which share their pages), so that
+    few CTAs would split each."""
+    from cybel_b200.kv_cache import PagedKVCache
+    from cybel_b200.paged_attention import RaggedBatch
+    import torch
+
+    seqs, n = 256, 2 ** 21
+    c = PagedKVCache(1, 1, n, batch=seqs, page_size=4096, q8=q8, n_slots=n // 4096)
+    c.table_host[...] = np.arange(n // 4096, dtype=np.int32)
+    c.sync_table()
+    g = torch.Generator(device="cuda")
+    g.manual_seed(1)
+    if q8:
+        c.k.random_(-127, 128)
+        c.v.random_(90, 128)
+        c.vs.fill_(0.01)
+    else:
+        c.k.normal_()
+        c.v.normal_(1.0, 0.1)
+    batch = RaggedBatch([1] * seqs, [n] * seqs)
+    q = _one_hot(seqs, 4, 128, 0.0625, g).half()
+    assert not _plan(q, batch, 1, q8=q8)[2]
+    out = c.attend(0, q, batch, scale=1.0)
+    _clean()
+    _check(c, 0, RaggedBatch([1], [n]), q[:1], out[:1], scale=1.0, terms=1)
