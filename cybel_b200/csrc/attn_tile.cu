@@ -33,8 +33,11 @@
 // much. So a product covers a step (head 64) or 64 positions and 64 columns of
 // the head (head 128) in an accumulator of its own, and the softmax warps add it
 // to the output, which costs 370 us instead of 267 at 4096 tokens and makes the
-// error 4e-7 instead of 2e-5 at 8000 positions. (fp16 rows keep the plain sum:
-// its error reaches that of their own rounding beyond 100 000 positions a CTA.)
+// error 4e-7 instead of 2e-5 at 8000 positions. Values of one sign lose more: 0.11 x
+// 2^-24 per position, 6.5e-3 over a million. fp16 rows keep the plain sum up to
+// 32768 positions a CTA (2e-4, under half of their own rounding's 4.9e-4); longer
+// ones are split further, and where eight CTAs do not reach, their products have
+// accumulators of their own, too (head 128: 64 columns at a time beside the weights).
 //
 // The output is rescaled in tensor memory by the softmax warps themselves and
 // only when a row's maximum rose by 2^kRise since the last time (fp32 rows: with
@@ -63,6 +66,7 @@ constexpr int kRows = 128;       // rows of a tile (MMA M), positions of a step 
 constexpr int kTiles = 2;
 constexpr int kCtaRows = kTiles * kRows;
 constexpr int kMaxCluster = 8;
+constexpr int kPlainSum = 32768;  // positions of a CTA whose sum the tensor cores keep (fp16 rows)
 constexpr int kBadWords = 64;    // steps whose values were cleaned, one bit each
 // Weights are 2^(score - reference maximum + kLift); the reference follows a
 // row's maximum once that has risen by kRise, so they stay below 2^15 in fp16.
@@ -215,17 +219,20 @@ __device__ __forceinline__ uint32_t clean16(uint32_t w) {
     return w;
 }
 
-template <int D, bool PREC, bool Q8>
+// PREC: fp32 rows (two parts). OWN: products have accumulators of their own.
+template <int D, bool PREC, bool OWN, bool Q8>
 __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const AttnArgs a) {
     using S = Tile<D, PREC, Q8>;
     using T = typename std::conditional<PREC, float, __half>::type;
     constexpr int NS = S::NS;
     constexpr int kMeta = S::kMeta;
     constexpr bool SC = Q8;  // scales beside the codes
-    // Where fp32 rows' products have accumulators of their own: of a whole step
-    // (head 64: tensor memory has room), or of 64 positions and columns at a time
-    // over the weights' place, which the next product has to wait for.
-    constexpr bool kWide = PREC && D == 64, kNarrow = PREC && D == 128;
+    static_assert(OWN || !PREC, "fp32 rows' products have accumulators of their own");
+    // Where they are: of a whole step (head 64: tensor memory has room), or of 64
+    // columns at a time (and 64 positions, where the weights have two parts) beside
+    // the weights, which the next product has to wait for.
+    constexpr bool kWide = OWN && D == 64, kNarrow = OWN && D == 128;
+    constexpr int kTurns = PREC ? 2 : 1;  // kNarrow: products of a step per 64 columns
     extern __shared__ __align__(1024) uint8_t smem[];
     Job* job_s = reinterpret_cast<Job*>(smem + S::kJob);
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + S::kJob + 120);
@@ -359,7 +366,7 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(issuer_regs(Q8)));
         if (warp < 12 + kTiles) {
             // ---------------- MMA issuer of tile t ----------------
-            constexpr uint32_t idS = idesc_of(kRows, false), idO = idesc_of(PREC ? 64 : D, true);
+            constexpr uint32_t idS = idesc_of(kRows, false), idO = idesc_of(kNarrow ? 64 : D, true);
             constexpr int kLast = S::kParts - 1;
             const int t = warp - 12;
             const Steps steps(sight, list, i0, job.lo[t], job.hi[t]);
@@ -380,7 +387,7 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
                     if (pv) {
                         const uint64_t v = v0 + ((vi % NS) * (S::kMat >> 4));
 #pragma unroll
-                        for (int half = 0; half < 2; ++half) {
+                        for (int half = 0; half < (kNarrow ? kTurns : 2); ++half) {
                             if constexpr (kNarrow) {
 #pragma unroll
                                 for (int d = 0; d < D / 64; ++d) {
@@ -389,9 +396,10 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
                                     tc_fence_after();
 #pragma unroll
                                     for (int k = 0; k < 8; ++k)  // low parts first
-                                        tc_mma_f16_ts(ts + 64, ts + (k < 4 ? 32 + k * 8 : (k - 4) * 8),
-                                                      v + d * (S::kHalf >> 4) + (4 * half + (k & 3)) * (2048 >> 4), idO,
-                                                      k > 0 ? 1u : 0u);
+                                        tc_mma_f16_ts(ts + 64, ts + (!PREC ? k * 8 : k < 4 ? 32 + k * 8 : (k - 4) * 8),
+                                                      v + d * (S::kHalf >> 4) +
+                                                          (PREC ? 4 * half + (k & 3) : k) * (2048 >> 4),
+                                                      idO, k > 0 ? 1u : 0u);
                                     tc_commit(pready(t, 1));
                                 }
                             } else {
@@ -700,7 +708,7 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
         const int t_lo = job.lo[t], t_hi = job.hi[t];
         float m = -INFINITY, l = 0.0f;
         float E = 0.0f, log_E = 0.0f;  // SC: the row's weights, their sum and its output are relative to E
-        // PREC: 64 columns of the output, o keep + the product at f (o 0 before `add`).
+        // OWN: 64 columns of the output, o keep + the product at f (o 0 before `add`).
         auto take = [&](uint32_t f, uint32_t o_at, bool add, float keep) {
 #pragma unroll
             for (int c = 0; c < 64; c += 16) {
@@ -857,7 +865,7 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
                     if (!(see[c >> 5] & (1u << (c & 31)))) x[c] = -INFINITY;
             }
             // ---- the reference maximum
-            float keep = 1.0f;  // PREC: what the output so far is worth from here on
+            float keep = 1.0f;  // OWN: what the output so far is worth from here on
             {
                 float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -872,7 +880,7 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
                     m = mn;
                     l *= f;
                     keep = f;
-                    if (!PREC && steps > 0) {
+                    if (!OWN && steps > 0) {
 #pragma unroll
                         for (int c = 0; c < D; c += 16) {
                             float o[16];
@@ -898,7 +906,8 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
             // ---- weights, a quarter of the positions at a time
             const float base = m == -INFINITY ? 0.0f : kLift - m - log_E + row_off;
             float2 s2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-            uint32_t parts[kNarrow ? 4 : 1][16];  // kNarrow: the second half's, kept until the first half's products are done
+            // kNarrow, two parts: the second half's, kept until the first half's products are done
+            uint32_t parts[kNarrow && PREC ? 4 : 1][16];
 #pragma unroll
             for (int quarter = 0; quarter < 4; ++quarter) {
                 if (quarter == 3 && lane == 0) mbar_arrive(next_turn);  // its first loads run under this one's tail
@@ -920,13 +929,13 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
                         lo16[c / 2] = pack2(p.x - h.x, p.y - h.y);
                     }
                 }
-                if (quarter == 2) {  // the first half has arrived in tensor memory long ago
+                if (quarter == 2 && !(kNarrow && !PREC)) {  // the first half has arrived in tensor memory long ago
                     tmem_wait_st();
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(pready(t, 0));
                 }
-                if constexpr (!kNarrow) {
+                if constexpr (!kNarrow || !PREC) {
                     tmem_st16(ts + quarter * 16, hi16);
                     if constexpr (PREC) tmem_st16(ts + 64 + quarter * 16, lo16);
                 } else if (quarter < 2) {
@@ -940,19 +949,28 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
             const float2 st = add2(s2[0], s2[1]);
             l += st.x + st.y;
             if constexpr (kNarrow) {
+                if constexpr (!PREC) {
+                    tmem_wait_st();
+                    tc_fence_before();
+                }
                 __syncwarp();
-                if (lane == 0) mbar_arrive(mempty(i));
+                if (lane == 0) {
+                    if constexpr (!PREC) mbar_arrive(pready(t, 0));
+                    mbar_arrive(mempty(i));
+                }
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
+                for (int half = 0; half < kTurns; ++half) {
 #pragma unroll
                     for (int d = 0; d < D / 64; ++d) {
                         ok = __all_sync(0xffffffffu, wait(pready(t, 1), drained++ & 1));
                         if (!ok) break;
                         tc_fence_after();
                         take(ts + 64, to + 64 * d, half > 0 || steps > 0, half > 0 ? 1.0f : keep);
-                        if (half == 0 && d == D / 64 - 1) {
+                        if constexpr (PREC) {
+                            if (half == 0 && d == D / 64 - 1) {
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) tmem_st16(ts + k * 16, parts[k]);
+                                for (int k = 0; k < 4; ++k) tmem_st16(ts + k * 16, parts[k]);
+                            }
                         }
                         tmem_wait_st();
                         tc_fence_before();
@@ -1095,8 +1113,8 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
     cluster_sync();  // no CTA leaves while another reads its shared memory
 }
 
-template <int D, bool PREC, bool Q8>
-int launch_tiles(const AttnArgs& a, long long total_rows, int max_kv, int sms, cudaStream_t st) {
+template <int D, bool PREC, bool OWN, bool Q8>
+int launch_tiles(const AttnArgs& a, long long units, int c, cudaStream_t st) {
     using S = Tile<D, PREC, Q8>;
     static std::mutex mu;
     static uint64_t done = 0;
@@ -1108,17 +1126,14 @@ int launch_tiles(const AttnArgs& a, long long total_rows, int max_kv, int sms, c
         if (!(done & bit)) {
             cudaFuncAttributes fa;
             // the register split adds up to 128 a thread: with fewer it would wait for ever
-            if (cudaFuncGetAttributes(&fa, b200q_attn_tile_kernel<D, PREC, Q8>) != cudaSuccess || fa.numRegs != 128 ||
-                cudaFuncSetAttribute(b200q_attn_tile_kernel<D, PREC, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     S::kTotal) != cudaSuccess)
+            if (cudaFuncGetAttributes(&fa, b200q_attn_tile_kernel<D, PREC, OWN, Q8>) != cudaSuccess ||
+                fa.numRegs != 128 ||
+                cudaFuncSetAttribute(b200q_attn_tile_kernel<D, PREC, OWN, Q8>,
+                                     cudaFuncAttributeMaxDynamicSharedMemorySize, S::kTotal) != cudaSuccess)
                 return B200Q_ECUDA;
             done |= bit;
         }
     }
-    const long long units = tile_blocks(a.r.batch, total_rows, a.most_rows, a.few_rows) * a.kv.n_kv;
-    if (units <= 0) return B200Q_OK;
-    const int c = tile_split(units, max_kv, sms);
-    if (units * c > 0x7fffffffll) return B200Q_ESHAPE;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(units * c));
     cfg.blockDim = dim3(kThreads);
@@ -1135,7 +1150,8 @@ int launch_tiles(const AttnArgs& a, long long total_rows, int max_kv, int sms, c
         attr[1].val.programmaticStreamSerializationAllowed = 1;
         cfg.numAttrs = 2;
     }
-    return cudaLaunchKernelEx(&cfg, b200q_attn_tile_kernel<D, PREC, Q8>, a) == cudaSuccess ? B200Q_OK : B200Q_ECUDA;
+    return cudaLaunchKernelEx(&cfg, b200q_attn_tile_kernel<D, PREC, OWN, Q8>, a) == cudaSuccess ? B200Q_OK
+                                                                                                : B200Q_ECUDA;
 }
 
 }  // namespace
@@ -1148,23 +1164,33 @@ long long tile_blocks(int batch, long long total_rows, int most_rows, int few_ro
 // While the blocks leave SMs idle, two steps a CTA at least (64 tokens of 32/8
 // heads at 2000 positions, fp16: 22 us, 30 with four), and eight CTAs only for
 // four fifths of the SMs: a GPC's are not a multiple of eight (16 clusters of
-// eight took 37 us at 4000 positions, of four 26).
-int tile_split(long long units, int max_kv, int sms) {
+// eight took 37 us at 4000 positions, of four 26). fp16 rows: more CTAs than that
+// before a CTA's sum passes kPlainSum (2048 tokens of 64/8 heads over 120 000
+// positions: 8.0 ms unsplit, 8.7 over four CTAs, 11.2 with sums in fp32; over
+// 250 000: 17.1, 21.6 over eight, 23.5; 1300 tokens of 32/1 heads over 120 000: 3.6,
+// 2.3, 5.6).
+int tile_split(long long units, int max_kv, int sms, bool fp32) {
     int c = 1;
     while (c < kMaxCluster && units * c * 2 <= (c * 2 < kMaxCluster ? sms : sms * 4 / 5) && max_kv >= c * 2 * 2 * kRows)
         c *= 2;
+    while (!fp32 && c < kMaxCluster && max_kv > c * kPlainSum) c *= 2;
     return c;
 }
 
 int launch_attn_tiles(const AttnArgs& a, int hd, bool fp32, bool q8, long long total_rows, int max_kv, int sms,
                       cudaStream_t st) {
-#define B200Q_TILES(D)                                                                 \
-    (fp32 ? (q8 ? launch_tiles<D, true, true>(a, total_rows, max_kv, sms, st)          \
-                : launch_tiles<D, true, false>(a, total_rows, max_kv, sms, st))        \
-          : (q8 ? launch_tiles<D, false, true>(a, total_rows, max_kv, sms, st)         \
-                : launch_tiles<D, false, false>(a, total_rows, max_kv, sms, st)))
+    const long long units = tile_blocks(a.r.batch, total_rows, a.most_rows, a.few_rows) * a.kv.n_kv;
+    if (units <= 0) return B200Q_OK;
+    const int c = tile_split(units, max_kv, sms, fp32);
+    if (units * c > 0x7fffffffll) return B200Q_ESHAPE;
+    const bool own = max_kv > c * kPlainSum;
+#define B200Q_TILES2(D, PREC, OWN) \
+    (q8 ? launch_tiles<D, PREC, OWN, true>(a, units, c, st) : launch_tiles<D, PREC, OWN, false>(a, units, c, st))
+#define B200Q_TILES(D) \
+    (fp32 ? B200Q_TILES2(D, true, true) : own ? B200Q_TILES2(D, false, true) : B200Q_TILES2(D, false, false))
     return hd == 128 ? B200Q_TILES(128) : B200Q_TILES(64);
 #undef B200Q_TILES
+#undef B200Q_TILES2
 }
 
 }  // namespace b200q

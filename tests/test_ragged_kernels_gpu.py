@@ -350,3 +350,56 @@ def test_a_step_over_two_million_positions(q8):
     out = c.attend(0, q, batch, scale=1.0)
     _clean()
     _check(c, 0, RaggedBatch([1], [n]), q[:1], out[:1], scale=1.0, terms=1)
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n,m,heads", [(100_000, 1300, 32), (1_000_000, 1300, 32), (1_000_000, 300, 4)])
+def test_sums_over_a_million_positions(n, m, heads, hd, q8):
+    """fp16 rows of a long prompt's chunk over contexts of a CTA's 100 000
+    positions and more, values of one sign."""
+    from cybel_b200.paged_attention import RaggedBatch
+
+    c, batch, g = _cache(([m], [n]), 1, hd, 4096, q8, seed=1)
+    if q8:
+        c.v.random_(90, 128)
+        c.vs.fill_(0.01)
+    else:
+        c.v.normal_(1.0, 0.1)
+    q = _one_hot(batch.n_tokens, heads, hd, 0.0625, g).half()
+    assert _plan(q, batch, 1, q8=q8)[2]
+    out = c.attend(0, q, batch, scale=1.0)
+    _clean()
+    for t in (0, m // 2, m - 1):
+        _check(c, 0, RaggedBatch([1], [n - m + t + 1]), q[t:t + 1], out[t:t + 1], scale=1.0, terms=1)
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_masks_beside_a_context_past_the_plain_sums(hd, q8):
+    """A context that eight CTAs cannot split into sums of 32768 positions: the
+    many-row kernel's fp16 rows add their products in fp32, here with a
+    window, a prefix, a cap and biases, for a long sequence and short ones."""
+    import torch
+
+    from cybel_b200.paged_attention import RaggedBatch
+
+    ql, kl, kv, heads = [700, 1, 300], [300_000, 500, 300], 2, 8
+    c, batch, g = _cache((ql, kl), kv, hd, 512, q8, seed=5)
+    q = _randn(batch, heads, hd, "fp16", g, 2.0)
+    prefix = torch.tensor([300, 40, 290], dtype=torch.int32, device="cuda")
+    slopes = torch.tensor([2.0 ** -(h + 1) for h in range(heads)], device="cuda")
+    for kw in (dict(window=1500), dict(window=1500, softcap=30.0), dict(window=200, slopes=slopes)):
+        assert _plan(q, batch, kv, prefix=1, q8=q8)[2:] != (0, 0)
+        out = c.attend(0, q, batch, prefix=prefix, **kw)
+        _clean()
+        ref = dict(window=kw["window"], cap=kw.get("softcap", 0.0), slopes=kw.get("slopes"))
+        at = 0
+        for b, (m, n) in enumerate(zip(ql, kl)):
+            for t in sorted({0, 1, m // 2, m - 1} & set(range(m))):
+                one = RaggedBatch([0] * b + [1], [0] * b + [n - m + t + 1])
+                pre = [0] * b + [int(prefix[b])]
+                if n - m + t + 1 < pre[b]:  # (positions of the prefix behind the row are not in this shorter view)
+                    continue
+                _check(c, 0, one, q[at + t:at + t + 1], out[at + t:at + t + 1], prefix=pre, **ref)
+            at += m
