@@ -41,7 +41,7 @@ int few_rows(int batch, int n_kv, long long total_rows, int most, int max_kv, bo
     const long long fw = (fu * fc + few_slots(sms) - 1) / few_slots(sms);
     const double few_us = 3.0 + static_cast<double>(fw) * (6.0 + (fp32 ? 0.018 : 0.021) * max_kv / fc);
     const long long tu = tile_blocks(batch, total_rows, most, 32) * n_kv;
-    const int tc = tile_split(tu, max_kv, sms, fp32);
+    const int tc = tile_split(tu, max_kv, sms);
     const long long steps = (max_kv + 128ll * tc - 1) / (128 * tc), tw = (tu * tc + sms - 1) / sms;
     const double step_us = fp32 ? (q8 ? 6.8 : 5.4) : (q8 ? 3.2 : 2.2);
     return few_us < (fp32 ? 16.0 : 11.0) + step_us * static_cast<double>(steps * tw) ? most : 32;
@@ -138,7 +138,7 @@ int attention_plan_info(int dtype, int n_tokens, int batch, int max_q_len, int m
     const long long blocks =
         p.most_rows > p.few_rows ? tile_blocks(batch, p.total_rows, p.most_rows, p.few_rows) * n_kv : 0;
     out[2] = blocks;
-    out[3] = blocks > 0 ? tile_split(blocks, p.reach, num_sms, fp32) : 0;
+    out[3] = blocks > 0 ? tile_split(blocks, p.reach, num_sms) : 0;
     return B200Q_OK;
 }
 

@@ -199,7 +199,7 @@ int launch_attn_tiles(const AttnArgs& a, int hd, bool fp32, bool q8, long long t
 // there are (the lengths are on the device) ...
 long long tile_blocks(int batch, long long total_rows, int most_rows, int few_rows);
 // ... and the CTAs that split the positions of each.
-int tile_split(long long units, int max_kv, int sms, bool fp32);
+int tile_split(long long units, int max_kv, int sms);
 // The few-row kernel's split of `units` blocks, and the CTAs that run at once.
 int few_split(long long units, int max_kv, int sms);
 int few_slots(int sms);

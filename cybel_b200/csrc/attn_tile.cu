@@ -1164,16 +1164,16 @@ long long tile_blocks(int batch, long long total_rows, int most_rows, int few_ro
 // While the blocks leave SMs idle, two steps a CTA at least (64 tokens of 32/8
 // heads at 2000 positions, fp16: 22 us, 30 with four), and eight CTAs only for
 // four fifths of the SMs: a GPC's are not a multiple of eight (16 clusters of
-// eight took 37 us at 4000 positions, of four 26). fp16 rows: more CTAs than that
-// before a CTA's sum passes kPlainSum (2048 tokens of 64/8 heads over 120 000
+// eight took 37 us at 4000 positions, of four 26). More CTAs than that before a
+// CTA's sum passes kPlainSum (fp16, 2048 tokens of 64/8 heads over 120 000
 // positions: 8.0 ms unsplit, 8.7 over four CTAs, 11.2 with sums in fp32; over
 // 250 000: 17.1, 21.6 over eight, 23.5; 1300 tokens of 32/1 heads over 120 000: 3.6,
-// 2.3, 5.6).
-int tile_split(long long units, int max_kv, int sms, bool fp32) {
+// 2.3, 5.6). fp32 sums' own roundings add up, too: 3e-6 at 100 000 positions a CTA.
+int tile_split(long long units, int max_kv, int sms) {
     int c = 1;
     while (c < kMaxCluster && units * c * 2 <= (c * 2 < kMaxCluster ? sms : sms * 4 / 5) && max_kv >= c * 2 * 2 * kRows)
         c *= 2;
-    while (!fp32 && c < kMaxCluster && max_kv > c * kPlainSum) c *= 2;
+    while (c < kMaxCluster && max_kv > c * kPlainSum) c *= 2;
     return c;
 }
 
@@ -1181,7 +1181,7 @@ int launch_attn_tiles(const AttnArgs& a, int hd, bool fp32, bool q8, long long t
                       cudaStream_t st) {
     const long long units = tile_blocks(a.r.batch, total_rows, a.most_rows, a.few_rows) * a.kv.n_kv;
     if (units <= 0) return B200Q_OK;
-    const int c = tile_split(units, max_kv, sms, fp32);
+    const int c = tile_split(units, max_kv, sms);
     if (units * c > 0x7fffffffll) return B200Q_ESHAPE;
     const bool own = max_kv > c * kPlainSum;
 #define B200Q_TILES2(D, PREC, OWN) \

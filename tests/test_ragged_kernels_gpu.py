@@ -352,12 +352,12 @@ def test_a_step_over_two_million_positions(q8):
     _check(c, 0, RaggedBatch([1], [n]), q[:1], out[:1], scale=1.0, terms=1)
 
 
-@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("dtype,q8", TYPES)
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("n,m,heads", [(100_000, 1300, 32), (1_000_000, 1300, 32), (1_000_000, 300, 4)])
-def test_sums_over_a_million_positions(n, m, heads, hd, q8):
-    """fp16 rows of a long prompt's chunk over contexts of a CTA's 100 000
-    positions and more, values of one sign."""
+def test_sums_over_a_million_positions(n, m, heads, hd, dtype, q8):
+    """A chunk of a long prompt whose blocks of rows fill the device, so that
+    their positions need no split for that: values of one sign."""
     from cybel_b200.paged_attention import RaggedBatch
 
     c, batch, g = _cache(([m], [n]), 1, hd, 4096, q8, seed=1)
@@ -366,7 +366,7 @@ def test_sums_over_a_million_positions(n, m, heads, hd, q8):
         c.vs.fill_(0.01)
     else:
         c.v.normal_(1.0, 0.1)
-    q = _one_hot(batch.n_tokens, heads, hd, 0.0625, g).half()
+    q = _one_hot(batch.n_tokens, heads, hd, 0.0625, g).to(_dt(dtype))
     assert _plan(q, batch, 1, q8=q8)[2]
     out = c.attend(0, q, batch, scale=1.0)
     _clean()
