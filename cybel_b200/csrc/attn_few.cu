@@ -25,7 +25,8 @@
 // Q8 rows enter as their integer codes, exact in fp16; a key's scale
 // multiplies its score, a value's scale its softmax weight, relative to a
 // power of two E above the scales that its row has seen so far, so that the
-// weight in fp16 neither over- nor underflows. Weights are kept 2^10 above 1 for the same reason.
+// weight in fp16 neither over- nor underflows. Weights are kept 2^10 above 1 for
+// the same reason.
 #include <algorithm>
 #include <mutex>
 #include <type_traits>
@@ -90,7 +91,8 @@ __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uin
 // error at 8000 positions is 3e-7 instead of 6e-6, for 1 to 3 percent of the time
 // (one row of 32/8 heads over 2048 positions 9.0 -> 9.2 us, 64 over 4000 175 -> 177;
 // Q8, the two parts joined at once, 110 -> 112; apart they spilled: 133).
-// fp16 rows (5 percent) take it, up to kPlainSum positions a warp.
+// fp16 rows, which it would cost 5 percent, keep the accumulator for up to kPlainSum
+// positions a warp.
 __device__ __forceinline__ void add4(float (&d)[4], const float (&t)[4]) {
     const float2 x = add2(make_float2(d[0], d[1]), make_float2(t[0], t[1]));
     const float2 y = add2(make_float2(d[2], d[3]), make_float2(t[2], t[3]));
@@ -475,7 +477,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) b200q_attn_few_kernel
 #pragma unroll
         for (int i2 = 0; i2 < NR; ++i2) {
             const float base = m[i2] == -INFINITY ? 0.0f : kLift - m[i2];
-            const float inv_E = __int_as_float(0x7F000000 - __float_as_int(E[i2]));  // (of a power of two, 2^126 at most)
+            // (of a power of two, 2^126 at most)
+            const float inv_E = __int_as_float(0x7F000000 - __float_as_int(E[i2]));
 #pragma unroll
             for (int f = 0; f < kTile / 16; ++f) {
                 float p[4];
@@ -554,8 +557,9 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) b200q_attn_few_kernel
 #pragma unroll
                     for (int t = 0; t < 4; ++t) {
                         const int r = 2 * c + (t & 1) + 8 * (t >> 1);
-                        const uint2 w = lds64(vt + (f * 16 + r) * F::RB + (D == 128 ? v_chunk<D, Q8>(r, g) * 16 + h * 8
-                                                                                   : v_chunk<D, Q8>(r, g >> 1) * 16 + (g & 1) * 8));
+                        const int at = D == 128 ? v_chunk<D, Q8>(r, g) * 16 + h * 8
+                                                : v_chunk<D, Q8>(r, g >> 1) * 16 + (g & 1) * 8;
+                        const uint2 w = lds64(vt + (f * 16 + r) * F::RB + at);
                         wv[f][t][0] = w.x ^ 0x80808080u, wv[f][t][1] = w.y ^ 0x80808080u;
                     }
 #pragma unroll

@@ -852,7 +852,8 @@ __global__ void __launch_bounds__(kThreads, 1) b200q_attn_tile_kernel(const Attn
                         row_off = -slope * (d0 - kEnd);
 #pragma unroll
                         for (int c = 0; c < kRows; c += 2)
-                            put2(x + c, fma2(both(slope), make_float2(c - kEnd, c + 1 - kEnd), make_float2(x[c], x[c + 1])));
+                            put2(x + c, fma2(both(slope), make_float2(c - kEnd, c + 1 - kEnd),
+                                             make_float2(x[c], x[c + 1])));
                     } else {
 #pragma unroll
                         for (int c = 0; c < kRows; ++c) x[c] = fmaf(-slope, fabsf(d0 - static_cast<float>(c)), x[c]);
